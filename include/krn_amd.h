@@ -139,6 +139,41 @@ int64_t krn_attention_workspace(int64_t bh, int64_t sq, int64_t sk, int64_t d, i
 int krn_softmax_rows(int kind, const void* x, void* y, int64_t rows, int64_t width, int64_t ldx, int64_t ldy,
                      void* stream);
 
+/* Microscaled 4-bit matrices (OCP MX, MXFP4). A row of k values is nb = ceil(k / 32) blocks of 32; `codes` holds 16 nb
+ * bytes a row, two e2m1 codes a byte with the first in the low nibble (sign in bit 3, magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6),
+ * and `scales` nb bytes a row, s standing for 2^(s - 127) and 255 for NaN. Both are row-major without padding; codes past k
+ * are zero; codes start at a 16-byte aligned address, scales at any. No counterpart in the reference, which has no 4-bit
+ * type.
+ *
+ * krn_mx_quantize: the MX matrix of `rows` rows of k values of kind KRN_F32, KRN_F16 or KRN_BF16. With E the biased float32
+ * exponent of a block's largest magnitude, s = max(E - 2, 0); a code is the e2m1 value nearest to x * 2^(127 - s), halves
+ * to even, 6 beyond 6. A block with a NaN or an infinity gets s = 255 and zero codes. krn_mx_dequantize: its values, rounded
+ * to the element kind (float32 and bf16 hold all finite ones). At most 2^31 blocks; values, codes and scales share no
+ * memory. */
+int krn_mx_quantize(int kind, const void* x, void* codes, void* scales, int64_t rows, int64_t k, void* stream);
+int krn_mx_dequantize(const void* codes, const void* scales, int kind, void* y, int64_t rows, int64_t k, void* stream);
+
+/* C[m, n] = epilogue(sum_k A[m, k] * B[n, k]) of two MX matrices, float32 sums; out_kind KRN_F32, KRN_F16 or KRN_BF16, the
+ * epilogue as for krn_gemm_nt. k is below 2^24, m and n below 2^31. C shares no memory with an operand. A workspace of
+ * krn_mx_gemm_workspace bytes (16-byte aligned, no preparation, not touched by other work until this call's has run; calls
+ * on one stream may share one) lets K be split over workgroups; with less, or none, another kernel runs. */
+int krn_mx_gemm(const void* a, const void* a_scales, const void* b, const void* b_scales, void* c, int out_kind, int64_t m,
+                int64_t n, int64_t k, int nops, const int* ops, const float* scalars, const void* const* vectors,
+                void* workspace, int64_t workspace_bytes, void* stream);
+int64_t krn_mx_gemm_workspace(int64_t m, int64_t n, int64_t k);
+
+/* A mixture-of-experts layer for `tokens` <= 64 tokens: y_t = sum over the top_k experts e of token t of
+ * w_te * down_e (silu(gate_e x_t) * up_e x_t). x is tokens x hidden and router experts x hidden, of kind KRN_F16 or KRN_BF16;
+ * a token's experts are those of the top_k largest x_t . router_e (ties to the lower index, NaN the largest), w_t the
+ * softmax of these logits. gate_up is the MX matrix of experts * 2 * inner rows of `hidden` values (an expert's gate rows,
+ * then its up rows), down that of experts * hidden rows of `inner` values. y is of x's kind and shares no memory with the
+ * inputs. At most 1024 experts, top_k <= 16. The workspace holds krn_moe_workspace bytes, needs no preparation, is 16-byte
+ * aligned and not touched by other work until this call's has run; calls on one stream may share one. */
+int krn_moe(int kind, const void* x, const void* router, const void* gate_up, const void* gate_up_scales, const void* down,
+            const void* down_scales, void* y, int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int64_t top_k,
+            void* workspace, int64_t workspace_bytes, void* stream);
+int64_t krn_moe_workspace(int kind, int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int64_t top_k);
+
 /* The message of the calling thread's last failed call. */
 const char* krn_amd_last_error(void);
 

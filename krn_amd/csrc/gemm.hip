@@ -1361,8 +1361,8 @@ static int gemm_dispatch(int fmt, bool nn, const void* a, const void* b, void* c
 
 // The epilogue chain of a launch, checked: at most four known operations, a vector for every per-row or per-column
 // one. `who` prefixes the error message.
-static bool epilogue_of(Epilogue& e, int out_kind, int nops, const int* ops, const float* scalars,
-                        const void* const* vectors, const char* who) {
+bool krn::epilogue_of(Epilogue& e, int out_kind, int nops, const int* ops, const float* scalars,
+                      const void* const* vectors, const char* who) {
   e.out_kind = out_kind;
   if (nops < 0 || nops > 4) {
     krn_set_error("%s: %d epilogue operations, at most 4", who, nops);

@@ -41,6 +41,10 @@ inline Epilogue plane_epilogue(int fmt) {
   return e;
 }
 
+// The epilogue chain of a launch, checked (gemm.hip); false with a message prefixed by `who`
+bool epilogue_of(Epilogue& e, int out_kind, int nops, const int* ops, const float* scalars, const void* const* vectors,
+                 const char* who);
+
 int launch_split(int fmt, bool nn, int shape, int parts, const SplitCall& g);
 int launch_reduce(int fmt, int parts, const SplitCall& g);
 

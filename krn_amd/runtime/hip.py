@@ -147,6 +147,16 @@ class HIPStream(Stream):
             held = self._workspace = self.device.empty_on(self, D.U8, nbytes)
         return held
 
+    def with_workspace(self, name: str, nbytes: int, call: Callable[[int, int], None]) -> None:
+        """`call(workspace, stream)` of the launch `name`. The call puts several kernels on the stream, each reading what
+        one before left in the workspace, and runs without the interpreter's lock: another thread's call must not put
+        its own between them."""
+        with self.workspace_lock:
+            workspace = self.workspace(nbytes)
+            call(workspace.pointer, self.handle)
+            recorded = workspace is not self._workspace and self.capturing
+            self.note(name, (workspace,) if recorded else ())
+
     @property
     def capturing(self) -> bool:
         return hipapi.capturing(self.handle)
@@ -412,18 +422,8 @@ class Launch:
         return self._with_workspace(product, need)
 
     def _with_workspace(self, call: Callable[[int, int], None], nbytes: int) -> Callable[[HIPStream], None]:
-        """`call(workspace, stream)` with the stream's workspace. The call puts two kernels on the stream, the second
-        reading what the first left in the workspace, and runs without the interpreter's lock: another thread's call
-        must not put its own between them."""
-
-        def run(stream: HIPStream) -> None:
-            with stream.workspace_lock:
-                workspace = stream.workspace(nbytes)
-                call(workspace.pointer, stream.handle)
-                recorded = workspace is not stream._workspace and stream.capturing
-                stream.note(self.kernel.name, (workspace,) if recorded else ())
-
-        return run
+        """`call(workspace, stream)` with the stream's workspace."""
+        return lambda stream: stream.with_workspace(self.kernel.name, nbytes, call)
 
     def _attention(self, plan: cdna4.AttentionPlan, params: dict, grid: Blocks):
         q, k, v, o = (params[n] for n in (plan.q, plan.k, plan.v, plan.o))

@@ -76,6 +76,24 @@ def lib() -> ctypes.CDLL:
     handle.krn_transpose16.argtypes = [c_void_p, c_void_p, c_int64, c_int64, c_void_p]
     handle.krn_softmax_rows.restype = c_int
     handle.krn_softmax_rows.argtypes = [c_int, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p]
+    handle.krn_mx_quantize.restype = c_int
+    handle.krn_mx_quantize.argtypes = [c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p]
+    handle.krn_mx_dequantize.restype = c_int
+    handle.krn_mx_dequantize.argtypes = [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_void_p]
+    handle.krn_mx_gemm.restype = c_int
+    handle.krn_mx_gemm.argtypes = [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, POINTER(c_int),
+        POINTER(c_float), POINTER(c_void_p), c_void_p, c_int64, c_void_p,
+    ]  # fmt: skip
+    handle.krn_mx_gemm_workspace.restype = c_int64
+    handle.krn_mx_gemm_workspace.argtypes = [c_int64, c_int64, c_int64]
+    handle.krn_moe.restype = c_int
+    handle.krn_moe.argtypes = [
+        c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
+        c_int64, c_void_p, c_int64, c_void_p,
+    ]  # fmt: skip
+    handle.krn_moe_workspace.restype = c_int64
+    handle.krn_moe_workspace.argtypes = [c_int, c_int64, c_int64, c_int64, c_int64, c_int64]
     return handle
 
 
@@ -185,3 +203,66 @@ def transpose16(src: int, dst: int, rows: int, cols: int, stream: int) -> None:
 def softmax_rows(dtype: Dtype, x: int, y: int, rows: int, width: int, ldx: int, ldy: int, stream: int) -> None:
     """y = softmax over the first `width` columns of each row of x (row strides ldx, ldy in elements)."""
     check(lib().krn_softmax_rows(kind(dtype), x, y, rows, width, ldx, ldy, stream), "krn_softmax_rows")
+
+
+def mx_quantize_call(dtype: Dtype, x: int, codes: int, scales: int, rows: int, k: int):
+    """The quantisation as a function of the stream, with the other arguments marshalled once."""
+    entry = lib().krn_mx_quantize
+    head = (c_int(kind(dtype)), c_void_p(x), c_void_p(codes), c_void_p(scales), c_int64(rows), c_int64(k))
+
+    def call(stream: int) -> None:
+        check(entry(*head, stream), "krn_mx_quantize")
+
+    return call
+
+
+def mx_dequantize_call(codes: int, scales: int, dtype: Dtype, y: int, rows: int, k: int):
+    """The values of an MX matrix as a function of the stream, with the other arguments marshalled once."""
+    entry = lib().krn_mx_dequantize
+    head = (c_void_p(codes), c_void_p(scales), c_int(kind(dtype)), c_void_p(y), c_int64(rows), c_int64(k))
+
+    def call(stream: int) -> None:
+        check(entry(*head, stream), "krn_mx_dequantize")
+
+    return call
+
+
+def mx_gemm_workspace(m: int, n: int, k: int) -> int:
+    """Bytes of device workspace `mx_gemm_call` of these sizes uses."""
+    return lib().krn_mx_gemm_workspace(m, n, k)
+
+
+def mx_gemm_call(a: tuple[int, int], b: tuple[int, int], c: int, out_dtype: Dtype, m: int, n: int, k: int,
+                 ops: list[tuple[int, float, int]], workspace_bytes: int):
+    """The product of two MX matrices, each (codes, scales), as a function of the workspace and the stream, with the
+    other arguments marshalled once."""
+    codes, scalars, vectors = marshal_ops(ops)
+    entry = lib().krn_mx_gemm
+    head = (c_void_p(a[0]), c_void_p(a[1]), c_void_p(b[0]), c_void_p(b[1]), c_void_p(c), c_int(kind(out_dtype)), c_int64(m),
+            c_int64(n), c_int64(k), c_int(len(ops)), codes, scalars, vectors)
+    size = c_int64(workspace_bytes)
+
+    def call(workspace: int, stream: int) -> None:
+        check(entry(*head, workspace, size, stream), "krn_mx_gemm")
+
+    return call
+
+
+def moe_workspace(dtype: Dtype, tokens: int, hidden: int, inner: int, experts: int, top_k: int) -> int:
+    """Bytes of device workspace `moe_call` of these sizes needs."""
+    return lib().krn_moe_workspace(kind(dtype), tokens, hidden, inner, experts, top_k)
+
+
+def moe_call(dtype: Dtype, x: int, router: int, gate_up: tuple[int, int], down: tuple[int, int], y: int, tokens: int,
+             hidden: int, inner: int, experts: int, top_k: int, workspace_bytes: int):
+    """The expert layer as a function of the workspace and the stream, with the other arguments marshalled once."""
+    entry = lib().krn_moe
+    head = (c_int(kind(dtype)), c_void_p(x), c_void_p(router), c_void_p(gate_up[0]), c_void_p(gate_up[1]),
+            c_void_p(down[0]), c_void_p(down[1]), c_void_p(y), c_int64(tokens), c_int64(hidden), c_int64(inner),
+            c_int64(experts), c_int64(top_k))
+    size = c_int64(workspace_bytes)
+
+    def call(workspace: int, stream: int) -> None:
+        check(entry(*head, workspace, size, stream), "krn_moe")
+
+    return call
