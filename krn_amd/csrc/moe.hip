@@ -171,11 +171,12 @@ __device__ __forceinline__ void split_f16(const u32x4& x, u32x4& hi, u32x4& lo) 
 // One lane's part of a slab of a weight row: blocks 4 j + g of it (j = 0 .. 3), and the row's scales
 struct WeightSlab {
   u32x4 code[4], scale;
-  __device__ void load(const uint8_t* codes, const uint8_t* scales, int block, int nb, int g) {
+  __device__ void load(const uint8_t* codes, const uint8_t* scales, int slab, int nb, int g) {
+    const int block = slab_block(slab, nb) + g;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      code[j] = block + 4 * j + g < nb ? *reinterpret_cast<const u32x4*>(codes + (int64_t)(block + 4 * j + g) * 16) : u32x4{};
-    scale = slab_scales(scales, block, nb);
+      code[j] = in_slab(block + 4 * j, slab, nb) ? *reinterpret_cast<const u32x4*>(codes + (int64_t)(block + 4 * j) * 16) : u32x4{};
+    scale = slab_scales(scales, slab, nb);
   }
   __device__ float factor(int j, int g) const { return __uint_as_float((scale[j] >> (8 * g) & 255u) << 23); }
 };
@@ -205,14 +206,15 @@ __global__ __launch_bounds__(256) void moe_up(const uint16_t* __restrict__ X, co
     if (i0 < I) {
       for (int s = from; s < to; ++s) {
         WeightSlab gc, uc;
-        gc.load(gw, gs, s * SLAB, nb, g);
-        uc.load(uw, us, s * SLAB, nb, g);
+        gc.load(gw, gs, s, nb, g);
+        uc.load(uw, us, s, nb, g);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float gf = gc.factor(j, g), uf = uc.factor(j, g);
+          const int block = slab_block(s, nb) + 4 * j + g;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const u32x4 v = eight16(x, ((int64_t)s * SLAB + 4 * j + g) * 32 + 8 * q, H);
+            const u32x4 v = in_slab(block, s, nb) ? eight16(x, (int64_t)block * 32 + 8 * q, H) : u32x4{};
             const u32x4 gv = bf16_codes(gc.code[j][q], gf), uv = bf16_codes(uc.code[j][q], uf);
             if constexpr (KIND == BF16) {
               gate = mfma16<BF16>(gv, v, gate), up = mfma16<BF16>(uv, v, up);
@@ -274,18 +276,18 @@ __global__ __launch_bounds__(512) void moe_down(const uint16_t* __restrict__ inn
       f32x4 acc = {};
       for (int s = from; s < to; ++s) {
         WeightSlab c;
-        c.load(w, sc, s * SLAB, nb, g);
+        c.load(w, sc, s, nb, g);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float factor = c.factor(j, g);
-          const int block = s * SLAB + 4 * j + g;
+          const int block = slab_block(s, nb) + 4 * j + g;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const u32x4 v = bf16_codes(c.code[j][q], factor);
             const int64_t from_x = (int64_t)block * 32 + 8 * q;
-            acc = mfma16<BF16>(v, block < nb ? *reinterpret_cast<const u32x4*>(x + from_x) : u32x4{}, acc);
+            acc = mfma16<BF16>(v, in_slab(block, s, nb) ? *reinterpret_cast<const u32x4*>(x + from_x) : u32x4{}, acc);
             if constexpr (KIND == F16)
-              acc = mfma16<BF16>(v, block < nb ? *reinterpret_cast<const u32x4*>(x + pairs * pitch + from_x) : u32x4{}, acc);
+              acc = mfma16<BF16>(v, in_slab(block, s, nb) ? *reinterpret_cast<const u32x4*>(x + pairs * pitch + from_x) : u32x4{}, acc);
           }
         }
       }

@@ -16,19 +16,36 @@ namespace krn {
 
 constexpr int MX_BLOCK = 32;
 constexpr int SLAB = 16;          // blocks of a slab
-constexpr uint32_t UNIT = 0x7f7f7f7f;  // four scales of 2^0
 
 __host__ __device__ inline int64_t mx_blocks(int64_t k) { return (k + MX_BLOCK - 1) / MX_BLOCK; }
 
-// The 16 scales of blocks `block` .. + 15 of a row of `nb`, 2^0 past its end (whose codes the callers make zero, so that
-// any finite scale does; a byte of the next row could be NaN)
-__device__ __forceinline__ u32x4 slab_scales(const uint8_t* row, int block, int nb) {
-  if (block + SLAB <= nb) return *reinterpret_cast<const u32x4_any*>(row + block);
-  u32x4 w = {UNIT, UNIT, UNIT, UNIT};
+// A row whose end cuts its last slab has that slab taken from its last 16 blocks: those of them that the slab before holds
+// already count as zeros there (the callers give their codes so), and the scales are 16 bytes of the row as they lie. (A
+// scale of 255 among the blocks taken twice makes both products NaN, as one does.) A row of fewer than 16 blocks is
+// one slab; its scales go byte by byte, 2^0 past its end, so that no byte outside the row is read.
+__device__ __forceinline__ int slab_block(int slab, int nb) { return nb < SLAB ? 0 : min(slab * SLAB, nb - SLAB); }
+
+// Whether block `block` counts in slab `slab` of a row of `nb` blocks
+__device__ __forceinline__ bool in_slab(int block, int slab, int nb) { return block >= slab * SLAB && block < nb; }
+
+__device__ __forceinline__ u32x4 long_scales(const uint8_t* row, int slab, int nb) {  // nb >= 16
+  return *reinterpret_cast<const u32x4_any*>(row + min(slab * SLAB, nb - SLAB));
+}
+
+__device__ __forceinline__ u32x4 short_scales(const uint8_t* row, int nb) {  // nb < 16
+  uint32_t b[SLAB];
 #pragma unroll
-  for (int i = 0; i < SLAB; ++i)
-    if (block + i < nb) w[i / 4] = (w[i / 4] & ~(0xffu << (8 * (i % 4)))) | (uint32_t)row[block + i] << (8 * (i % 4));
+  for (int i = 0; i < SLAB; ++i) b[i] = row[min(i, nb - 1)];
+#pragma unroll
+  for (int i = 0; i < SLAB; ++i) b[i] = i < nb ? b[i] : 0x7f;
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = b[4 * i] | b[4 * i + 1] << 8 | b[4 * i + 2] << 16 | b[4 * i + 3] << 24;
   return w;
+}
+
+__device__ __forceinline__ u32x4 slab_scales(const uint8_t* row, int slab, int nb) {
+  return nb < SLAB ? short_scales(row, nb) : long_scales(row, slab, nb);
 }
 
 // Byte g of each of four words, in one word

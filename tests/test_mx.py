@@ -156,7 +156,7 @@ def test_the_entry_points_refuse_before_any_device_call():
     assert "aligned" in product(a=p((1 << 30) + 4))
     assert "shares memory" in product(c=codes)
     assert "shares memory" in product(c=p((1 << 32) - 1))
-    assert "2^24" in product(k=1 << 24) and "2^24" in product(k=0) and "2^24" in product(m=-1)
+    assert "2^23" in product(k=1 << 23) and "2^23" in product(k=0) and "2^23" in product(m=-1)
     assert "2^24 tiles" in product(m=(1 << 31) - 1, n=1 << 20)
     assert "at most 4" in product(nops=5)
     assert "unknown epilogue" in product(nops=1, ops=(ctypes.c_int * 1)(9))
