@@ -4,15 +4,16 @@
 // counts as the largest.
 //
 // Bound by reading the chosen experts' weights, each once whatever the number of its tokens (up to 16). Four launches:
-//   logits  x router^T in 16-bit MFMAs (products exact, float32 sums), K split over workgroups, partial sums to memory
+//   logits  x router^T in 16-bit MFMAs (products exact, float32 sums)
 //   route   one workgroup: a wave chooses a token's experts; every expert's tokens as a 64-bit mask, so that its count and a
 //           token's place in it are population counts and no order of atomics shows; the chosen experts in a row
-//   up      a workgroup per 16 inner values of a chosen expert: gate and up rows, silu(gate) * up * w to memory in bf16
+//   up      16 inner values of a chosen expert a wave: gate and up rows, w silu(gate) up to memory
 //   down    a workgroup per 16 outputs: all chosen experts' rows, added per token
 // Weights go to bf16 exactly (v_cvt_scalef32_pk_bf16_fp4: two bits of mantissa and a power of two) and are multiplied in
-// 16x16x32 bf16 MFMAs, 16 weight rows by up to 16 tokens. bfloat16 tokens are taken as they are and the inner values
-// rounded to bfloat16, as a bf16 layer stores them; float16 tokens and their inner values are split into a bf16 and
-// the bf16 of the remainder, which holds all of a float16, so that nothing is lost and nothing overflows.
+// 16x16x32 bf16 MFMAs, 16 weight rows by up to 16 tokens. bfloat16 tokens are taken as they are; float16 tokens are split
+// into the nearest bf16 and the bf16 of what is left, which holds all of a float16. The inner values are handed on as two
+// such parts for both types, 2^-16 relative: one bf16 would add as much error as the result's own rounding (1 token of
+// 4096: 2.4e-3 against 1.7e-3), and the second MFMA hides behind the weights' way from memory.
 #include "mx_parts.h"
 
 namespace krn {
@@ -45,21 +46,31 @@ __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, f32x4 c)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Partial logits of 16 experts and 16 tokens over the K steps of part blockIdx.z: partial[part][token][expert]
+// Logits of 16 experts and 16 tokens over one of PARTS runs of K (blockIdx.z), which its four waves split again
+constexpr int PARTS = 8;
 template <int KIND>
 __global__ __launch_bounds__(256) void moe_logits(const uint16_t* __restrict__ X, const uint16_t* __restrict__ router,
-                                                  float* __restrict__ partial, int T, int64_t H, int E, int steps) {
+                                                  float* __restrict__ partial, int T, int64_t H, int E) {
   __shared__ f32x4 sums[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const int e0 = blockIdx.x * 16, t0 = blockIdx.y * 16;
-  const uint16_t* w = router + (int64_t)min(e0 + r, E - 1) * H;
-  const uint16_t* x = X + (int64_t)min(t0 + r, T - 1) * H;
+  const int e0 = blockIdx.x * 16, t0 = blockIdx.y * 16, run = blockIdx.z * 4 + wave;
+  const uint16_t* w = router + (int64_t)min(e0 + r, E - 1) * H + 8 * g;
+  const uint16_t* x = X + (int64_t)min(t0 + r, T - 1) * H + 8 * g;
   f32x4 acc = {};
-  const int64_t first = ((int64_t)blockIdx.z * 4 + wave) * steps * 32;
-  for (int s = 0; s < steps; ++s) {
-    const int64_t at = first + s * 32 + g * 8;
-    acc = mfma16<KIND>(eight16(w, at, H), eight16(x, at, H), acc);
+  const int steps = (int)((H + 31) / 32), whole = (int)(H / 32);
+  const int to = (int)((int64_t)steps * (run + 1) / (4 * PARTS));
+  int s = (int)((int64_t)steps * run / (4 * PARTS));
+  for (; s + 4 <= min(to, whole); s += 4) {
+    u32x4 a[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = *reinterpret_cast<const u32x4_any*>(w + (s + i) * 32);
+      b[i] = *reinterpret_cast<const u32x4_any*>(x + (s + i) * 32);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc = mfma16<KIND>(a[i], b[i], acc);
   }
+  for (; s < to; ++s) acc = mfma16<KIND>(eight16(w, s * 32, H - 8 * g), eight16(x, s * 32, H - 8 * g), acc);
   sums[wave][lane] = acc;
   __syncthreads();
   if (wave == 0 && t0 + r < T) {
@@ -70,6 +81,18 @@ __global__ __launch_bounds__(256) void moe_logits(const uint16_t* __restrict__ X
   }
 }
 
+// The largest (smallest) of a wave's values, in every lane: four DPP steps within 16 lanes, then the four rows' results
+template <bool MAX>
+__device__ __forceinline__ uint32_t wave_extreme(uint32_t v) {
+  auto pick = [](uint32_t a, uint32_t b) { return MAX ? max(a, b) : min(a, b); };
+  v = pick(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true));   // lane ^ 1
+  v = pick(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));   // lane ^ 2
+  v = pick(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, true));  // half row mirrored
+  v = pick(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, true));  // row mirrored
+  return pick(pick((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16)),
+              pick((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48)));
+}
+
 // A float32 as an unsigned number in the same order, never 0; NaN above everything
 __device__ __forceinline__ uint32_t ordered(float x) {
   if (x != x) return 0xffffffffu;
@@ -77,9 +100,9 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__global__ __launch_bounds__(1024) void moe_route(const float* __restrict__ partial, int parts, int T, int E, int top_k,
-                                                  Routing out) {
-  __shared__ uint32_t key[16][MOE_EXPERTS];  // a wave's token's logits in order, 0 once chosen
+// EPL: experts a lane
+template <int EPL>
+__global__ __launch_bounds__(1024) void moe_route(const float* __restrict__ partial, int T, int E, int top_k, Routing out) {
   __shared__ unsigned long long mask[MOE_EXPERTS];
   __shared__ uint32_t base[MOE_EXPERTS], wave_sum[16];
   __shared__ int chosen[MOE_TOKENS * MOE_TOP_K];
@@ -88,28 +111,32 @@ __global__ __launch_bounds__(1024) void moe_route(const float* __restrict__ part
   mask[threadIdx.x] = 0;
   __syncthreads();
   for (int t = wave; t < T; t += 16) {
-    for (int e = lane; e < E; e += 64) {
-      float v = 0.0f;
-      for (int p = 0; p < parts; ++p) v += partial[((int64_t)p * T + t) * E + e];
-      key[wave][e] = ordered(v);
+    uint32_t key[EPL];  // expert lane + 64 i, 0 once chosen and past the last
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const int e = lane + 64 * i;
+      float v[PARTS];
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) v[p] = partial[((int64_t)p * T + t) * E + min(e, E - 1)];
+      float sum = v[0];
+#pragma unroll
+      for (int p = 1; p < PARTS; ++p) sum += v[p];
+      key[i] = e < E ? ordered(sum) : 0;
     }
     float mine = -INFINITY;  // lane j: the logit of choice j
     int pick = 0;
     for (int j = 0; j < top_k; ++j) {
-      unsigned long long best = 0;
-      for (int e = lane; e < E; e += 64) {
-        const unsigned long long v = (unsigned long long)key[wave][e] << 32 | (uint32_t)~e;
-        best = v > best ? v : best;
-      }
+      uint32_t best = key[0];
 #pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const unsigned long long v = __shfl_xor(best, d);
-        best = v > best ? v : best;
-      }
-      const int e = (int)~(uint32_t)best;
-      const uint32_t u = (uint32_t)(best >> 32);
-      if (lane == j) mine = __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u), pick = e;
-      if (lane == (e & 63)) key[wave][e] = 0;
+      for (int i = 1; i < EPL; ++i) best = max(best, key[i]);
+      best = wave_extreme<true>(best);
+      uint32_t e = MOE_EXPERTS;  // the lowest expert with that logit
+#pragma unroll
+      for (int i = EPL - 1; i >= 0; --i) e = key[i] == best ? lane + 64 * i : e;
+      e = wave_extreme<false>(e);
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) key[i] = lane + 64 * i == (int)e ? 0 : key[i];
+      if (lane == j) mine = __uint_as_float(best & 0x80000000u ? best ^ 0x80000000u : ~best), pick = (int)e;
     }
     const float top = __shfl(mine, 0);
     const float p = lane < top_k ? expf(mine - top) : 0.0f;
@@ -158,13 +185,19 @@ __device__ __forceinline__ u32x4 bf16_codes(uint32_t w, float scale) {
                __builtin_bit_cast(uint32_t, d)};
 }
 
+// What is left of a value when its bf16 is taken away; nothing of one that is, or becomes, infinite
+__device__ __forceinline__ float rest(float v, uint16_t bf) {
+  const float h = bf2f(bf);
+  return __builtin_isinf(h) ? 0.0f : v - h;
+}
+
 // Eight float16 values as the bf16 nearest to each and the bf16 of what is left (exact: 11 bits in two times 8)
 __device__ __forceinline__ void split_f16(const u32x4& x, u32x4& hi, u32x4& lo) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float a = h2f((uint16_t)x[i]), b = h2f((uint16_t)(x[i] >> 16));
     hi[i] = f2bf2(a, b);
-    lo[i] = f2bf2(a - bf2f((uint16_t)hi[i]), b - bf2f((uint16_t)(hi[i] >> 16)));
+    lo[i] = f2bf2(rest(a, (uint16_t)hi[i]), rest(b, (uint16_t)(hi[i] >> 16)));
   }
 }
 
@@ -183,125 +216,179 @@ struct WeightSlab {
 
 __device__ __forceinline__ float silu_times(float gate, float up) { return gate / (1.0f + expf(-gate)) * up; }
 
-// Inner values i0 .. i0 + 15 of the chosen expert blockIdx.y, for its tokens, 16 at a time: lane (r, q) row r of the 16 gate
-// and up rows. Four waves split the slabs. Past the inner size, up to whole blocks, zeros.
+// Tokens' values for one slab in LDS, where the waves take their MFMA operands from: a row of 512 values is 1024 bytes, and
+// rows lie 1040 apart, so that the 16 rows a read touches are on different banks. A token's slab is one access of
+// a wave to memory; as operands straight from memory it would be 16, whatever the number of tokens, and the address
+// path would bound the kernel (down, 16 tokens of 4: 127 us).
+constexpr int STAGED_ROW = 1040;
+
+// Operand (j, q) of lane (r, g): values 8 q .. + 7 of block 4 j + g of the slab, of row min(r, rows - 1)
+__device__ __forceinline__ u32x4 staged(const uint8_t* slab, int row, int j, int q, int g) {
+  return *reinterpret_cast<const u32x4*>(slab + row * STAGED_ROW + (4 * j + g) * 64 + q * 16);
+}
+
+// Inner values of the chosen expert blockIdx.y for its tokens, `rows` (at most 16) at a time. Eight waves: `kparts` of them
+// split the slabs of 16 gate and 16 up rows, so that a workgroup has 8 / kparts times 16 inner values. Past the
+// inner size, up to whole blocks, zeros. Dynamic LDS: kparts slabs of `rows` tokens (float16: of both parts).
 template <int KIND>
-__global__ __launch_bounds__(256) void moe_up(const uint16_t* __restrict__ X, const uint8_t* __restrict__ W,
+__global__ __launch_bounds__(512) void moe_up(const uint16_t* __restrict__ X, const uint8_t* __restrict__ W,
                                               const uint8_t* __restrict__ S, uint16_t* __restrict__ inner, Routing route,
-                                              int64_t H, int I, int pairs) {
-  __shared__ f32x4 sums[4][2][64];
+                                              int64_t H, int I, int pairs, int kparts, int rows) {
+  constexpr int PLANES = KIND == F16 ? 2 : 1;
+  extern __shared__ __attribute__((aligned(16))) uint8_t tokens[];
+  __shared__ f32x4 sums[8][2][64];
   const int a = blockIdx.y;
   if (a >= route.active[0]) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int e = route.active[1 + a], begin = route.offset[a], count = route.offset[a + 1] - begin;
-  const int i0 = blockIdx.x * 16, nb = (int)mx_blocks(H), slabs = (nb + SLAB - 1) / SLAB;
+  const int part = wave % kparts, i0 = (blockIdx.x * (8 / kparts) + wave / kparts) * 16;
+  const int nb = (int)mx_blocks(H), slabs = (nb + SLAB - 1) / SLAB;
   const int64_t pitch = mx_blocks(I) * MX_BLOCK, row = (int64_t)e * 2 * I + min(i0 + r, I - 1);
   const uint8_t *gw = W + row * nb * 16, *uw = W + (row + I) * nb * 16, *gs = S + row * nb, *us = S + (row + I) * nb;
-  const int from = slabs * wave / 4, to = slabs * (wave + 1) / 4;
-  for (int f = 0; f < count; f += 16) {
-    const int at = begin + min(f + r, count - 1), t = route.token[at];
-    const float weight = route.weight[at];
-    const uint16_t* x = X + (int64_t)t * H;
+  const int plane = kparts * rows * STAGED_ROW;
+  const uint8_t* mine = tokens + part * rows * STAGED_ROW;
+  for (int f = 0; f < count; f += rows) {
+    const int here = min(count - f, rows), own = min(r, here - 1);
     f32x4 gate = {}, up = {};
-    if (i0 < I) {
-      for (int s = from; s < to; ++s) {
-        WeightSlab gc, uc;
-        gc.load(gw, gs, s, nb, g);
-        uc.load(uw, us, s, nb, g);
+    for (int from = 0; from < slabs; from += kparts) {
+      const int slab = from + part;
+      const bool work = slab < slabs && i0 < I;
+      WeightSlab gc, uc;
+      if (work) gc.load(gw, gs, slab, nb, g), uc.load(uw, us, slab, nb, g);
+      if (from > 0 || f > 0) __syncthreads();  // the tokens before have been read
+      for (int i = wave; i < here * kparts; i += 8) {
+        const int s = from + i % kparts, t = i / kparts, block = slab_block(s, nb) + (lane >> 2);
+        if (s >= slabs) continue;
+        const u32x4 v = in_slab(block, s, nb) ? eight16(X + (int64_t)route.token[begin + f + t] * H,
+                                                        (int64_t)block * 32 + 8 * (lane & 3), H)
+                                              : u32x4{};
+        uint8_t* to = tokens + ((i % kparts) * rows + t) * STAGED_ROW + lane * 16;
+        if constexpr (KIND == F16) {
+          u32x4 hi, lo;
+          split_f16(v, hi, lo);
+          *reinterpret_cast<u32x4*>(to) = hi, *reinterpret_cast<u32x4*>(to + plane) = lo;
+        } else {
+          *reinterpret_cast<u32x4*>(to) = v;
+        }
+      }
+      __syncthreads();
+      if (!work) continue;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float gf = gc.factor(j, g), uf = uc.factor(j, g);
-          const int block = slab_block(s, nb) + 4 * j + g;
+      for (int j = 0; j < 4; ++j) {
+        const float gf = gc.factor(j, g), uf = uc.factor(j, g);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const u32x4 v = in_slab(block, s, nb) ? eight16(x, (int64_t)block * 32 + 8 * q, H) : u32x4{};
-            const u32x4 gv = bf16_codes(gc.code[j][q], gf), uv = bf16_codes(uc.code[j][q], uf);
-            if constexpr (KIND == BF16) {
-              gate = mfma16<BF16>(gv, v, gate), up = mfma16<BF16>(uv, v, up);
-            } else {
-              u32x4 hi, lo;
-              split_f16(v, hi, lo);
-              gate = mfma16<BF16>(gv, hi, gate), up = mfma16<BF16>(uv, hi, up);
-              gate = mfma16<BF16>(gv, lo, gate), up = mfma16<BF16>(uv, lo, up);
-            }
+        for (int q = 0; q < 4; ++q) {
+          const u32x4 gv = bf16_codes(gc.code[j][q], gf), uv = bf16_codes(uc.code[j][q], uf);
+#pragma unroll
+          for (int p = 0; p < PLANES; ++p) {
+            const u32x4 v = staged(mine + p * plane, own, j, q, g);
+            gate = mfma16<BF16>(gv, v, gate), up = mfma16<BF16>(uv, v, up);
           }
         }
       }
     }
     sums[wave][0][lane] = gate, sums[wave][1][lane] = up;
     __syncthreads();
-    if (wave == 0 && f + r < count) {
-      gate = (sums[0][0][lane] + sums[1][0][lane]) + (sums[2][0][lane] + sums[3][0][lane]);
-      up = (sums[0][1][lane] + sums[1][1][lane]) + (sums[2][1][lane] + sums[3][1][lane]);
+    if (part == 0 && r < here && i0 < pitch) {
+      for (int p = 1; p < kparts; ++p) gate += sums[wave + p][0][lane], up += sums[wave + p][1][lane];
+      const float weight = route.weight[begin + f + r];
       float v[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) v[q] = i0 + 4 * g + q < I ? silu_times(gate[q], up[q]) * weight : 0.0f;
       uint16_t* out = inner + (int64_t)(begin + f + r) * pitch + i0 + 4 * g;
       const uint32_t h0 = f2bf2(v[0], v[1]), h1 = f2bf2(v[2], v[3]);
+      const uint32_t l0 = f2bf2(rest(v[0], (uint16_t)h0), rest(v[1], (uint16_t)(h0 >> 16)));
+      const uint32_t l1 = f2bf2(rest(v[2], (uint16_t)h1), rest(v[3], (uint16_t)(h1 >> 16)));
       *reinterpret_cast<u32x2*>(out) = u32x2{h0, h1};
-      if constexpr (KIND == F16) {
-        const uint32_t l0 = f2bf2(v[0] - bf2f((uint16_t)h0), v[1] - bf2f((uint16_t)(h0 >> 16)));
-        const uint32_t l1 = f2bf2(v[2] - bf2f((uint16_t)h1), v[3] - bf2f((uint16_t)(h1 >> 16)));
-        *reinterpret_cast<u32x2*>(out + pairs * pitch) = u32x2{l0, l1};
-      }
+      *reinterpret_cast<u32x2*>(out + pairs * pitch) = u32x2{l0, l1};
     }
-    __syncthreads();
   }
 }
 
-// Outputs n0 .. n0 + 15 of every token: the eight waves split the chosen experts' slabs, each adding an expert's part for
-// its tokens into sums of its own, which meet at the end in the order of the waves.
-template <int KIND>
+// Outputs n0 .. n0 + 255 of every token over part blockIdx.y of the chosen experts' slabs: each of the eight waves has 32
+// weight rows and goes through all of the part, its next slab's weights on their way; the waves share the inner values in
+// LDS, two slabs' places in turn. An expert's part goes to its tokens' sums, which only the wave with those rows touches.
+// Dynamic LDS: two slabs of `rows` tokens (at most 16) in two parts, then the sums of T tokens.
 __global__ __launch_bounds__(512) void moe_down(const uint16_t* __restrict__ inner, const uint8_t* __restrict__ W,
-                                                const uint8_t* __restrict__ S, uint16_t* __restrict__ Y, Routing route,
-                                                int T, int64_t H, int I, int pairs) {
-  constexpr int WAVES = 8;
-  __shared__ f32x4 sums[WAVES][MOE_TOKENS][4];
+                                                const uint8_t* __restrict__ S, float* __restrict__ partial, Routing route,
+                                                int T, int64_t H, int I, int pairs, int rows) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t tokens[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-  const int64_t n0 = (int64_t)blockIdx.x * 16;
-  for (int i = lane; i < T * 4; i += 64) sums[wave][i >> 2][i & 3] = f32x4{};
+  const int plane = rows * STAGED_ROW;
+  f32x4* sums = reinterpret_cast<f32x4*>(tokens + 4 * plane) + wave * 8;  // [token][64], this wave's eight
+  const int64_t n0 = (int64_t)blockIdx.x * 256 + wave * 32;
+  for (int i = lane; i < T * 8; i += 64) sums[(i >> 3) * 64 + (i & 7)] = f32x4{};
   const int nb = (int)mx_blocks(I), slabs = (nb + SLAB - 1) / SLAB, items = route.active[0] * slabs;
   const int64_t pitch = (int64_t)nb * MX_BLOCK;
-  int item = items * wave / WAVES;
-  const int end = items * (wave + 1) / WAVES;
-  while (item < end) {
-    const int a = item / slabs, from = item - a * slabs, to = min(slabs, from + end - item);
-    item += to - from;
-    const int begin = route.offset[a], count = route.offset[a + 1] - begin;
-    const int64_t row = (int64_t)route.active[1 + a] * H + min(n0 + r, H - 1);
-    const uint8_t *w = W + row * nb * 16, *sc = S + row * nb;
-    for (int f = 0; f < count; f += 16) {
-      const int at = begin + min(f + r, count - 1);
-      const uint16_t* x = inner + at * pitch;
-      f32x4 acc = {};
-      for (int s = from; s < to; ++s) {
-        WeightSlab c;
-        c.load(w, sc, s, nb, g);
+  const int first = (int)((int64_t)items * blockIdx.y / gridDim.y), end = (int)((int64_t)items * (blockIdx.y + 1) / gridDim.y);
+  auto load = [&](WeightSlab (&w)[2], int item) {
+    const int a = item / slabs;
+    const int64_t expert = route.active[1 + a] * H;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float factor = c.factor(j, g);
-          const int block = slab_block(s, nb) + 4 * j + g;
+    for (int i = 0; i < 2; ++i) {
+      const int64_t at = (expert + min(n0 + 16 * i + r, H - 1)) * nb;
+      w[i].load(W + at * 16, S + at, item - a * slabs, nb, g);
+    }
+  };
+  WeightSlab now[2];
+  if (first < end) load(now, first);
+  int place = 0;
+  for (int item = first; item < end; ++item) {
+    WeightSlab next[2] = {now[0], now[1]};
+    if (item + 1 < end) load(next, item + 1);
+    const int a = item / slabs, s = item - a * slabs, begin = route.offset[a], count = route.offset[a + 1] - begin;
+    for (int f = 0; f < count; f += rows) {
+      const int here = min(count - f, rows), own = min(r, here - 1);
+      uint8_t* at = tokens + place * 2 * plane;
+      place ^= 1;
+      for (int i = wave; i < 2 * here; i += 8) {
+        const int t = i >> 1, block = slab_block(s, nb) + (lane >> 2);
+        const uint16_t* from = inner + ((i & 1) * pairs + begin + f + t) * pitch + (int64_t)block * 32 + 8 * (lane & 3);
+        *reinterpret_cast<u32x4*>(at + (i & 1) * plane + t * STAGED_ROW + lane * 16) =
+            in_slab(block, s, nb) ? *reinterpret_cast<const u32x4*>(from) : u32x4{};
+      }
+      __syncthreads();  // and every wave is done with what was in this place two slabs ago
+      f32x4 acc[2] = {};
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const u32x4 v = bf16_codes(c.code[j][q], factor);
-            const int64_t from_x = (int64_t)block * 32 + 8 * q;
-            acc = mfma16<BF16>(v, in_slab(block, s, nb) ? *reinterpret_cast<const u32x4*>(x + from_x) : u32x4{}, acc);
-            if constexpr (KIND == F16)
-              acc = mfma16<BF16>(v, in_slab(block, s, nb) ? *reinterpret_cast<const u32x4*>(x + pairs * pitch + from_x) : u32x4{}, acc);
+      for (int j = 0; j < 4; ++j) {
+        const float f0 = now[0].factor(j, g), f1 = now[1].factor(j, g);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const u32x4 v0 = bf16_codes(now[0].code[j][q], f0), v1 = bf16_codes(now[1].code[j][q], f1);
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const u32x4 v = staged(at + p * plane, own, j, q, g);
+            acc[0] = mfma16<BF16>(v0, v, acc[0]), acc[1] = mfma16<BF16>(v1, v, acc[1]);
           }
         }
       }
-      if (f + r < count) sums[wave][route.token[at]][g] += acc;
+      if (r < here) {
+        f32x4* sum = sums + route.token[begin + f + r] * 64 + g;
+        sum[0] += acc[0], sum[4] += acc[1];
+      }
     }
+    now[0] = next[0], now[1] = next[1];
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < T * 16; i += WAVES * 64) {
-    const int t = i >> 4, n = i & 15;
-    float v = 0.0f;
+  for (int i = lane; i < T * 8; i += 64) {
+    const int t = i >> 3;
+    const f32x4 v = sums[t * 64 + (i & 7)];
+    float* out = partial + ((int64_t)blockIdx.y * T + t) * H + n0 + 4 * (i & 7);
 #pragma unroll
-    for (int s = 0; s < WAVES; ++s) v += reinterpret_cast<const float*>(&sums[s][t][0])[n];
-    if (n0 + n < H) Y[(int64_t)t * H + n0 + n] = KIND == BF16 ? f2bf(v) : f2h(v);
+    for (int q = 0; q < 4; ++q)
+      if (n0 + 4 * (i & 7) + q < H) out[q] = v[q];
   }
+}
+
+// y = the sum of the parts, in their order
+template <int KIND>
+__global__ __launch_bounds__(256) void moe_sum(const float* __restrict__ partial, uint16_t* __restrict__ Y, int64_t values,
+                                               int parts) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= values) return;
+  float v = 0.0f;
+#pragma unroll 8
+  for (int p = 0; p < parts; ++p) v += partial[p * values + i];
+  Y[i] = KIND == BF16 ? f2bf(v) : f2h(v);
 }
 
 }  // namespace krn
@@ -311,26 +398,27 @@ using namespace krn;
 namespace {
 
 struct Layout {  // of the workspace, in bytes
-  int parts, steps;
-  int64_t partial, active, offset, token, weight, inner, bytes;
+  int parts;  // of the down products, so that their workgroups fill the chip
+  int64_t logits, active, offset, token, weight, inner, partial, bytes;
 };
 
-Layout layout_of(int kind, int64_t t, int64_t h, int64_t i, int64_t experts, int64_t top_k) {
+Layout layout_of(int64_t t, int64_t h, int64_t i, int64_t experts, int64_t top_k) {
   Layout w{};
-  const int64_t steps = (h + 31) / 32, pairs = t * top_k;
-  w.steps = steps <= 256 ? 4 : (int)((steps + 63) / 64);  // of each of a workgroup's four waves
-  w.parts = (int)((steps + 4 * w.steps - 1) / (4 * w.steps));
+  const int64_t pairs = t * top_k, most = pairs < experts ? pairs : experts, blocks = (h + 255) / 256;
+  const int64_t items = most * ((mx_blocks(i) + SLAB - 1) / SLAB), fill = (256 + blocks - 1) / blocks;
+  w.parts = (int)(items < fill ? items : fill);
   auto take = [&](int64_t bytes) {
     const int64_t at = w.bytes;
     w.bytes += (bytes + 255) / 256 * 256;
     return at;
   };
-  w.partial = take(w.parts * t * experts * 4);
+  w.logits = take(PARTS * t * experts * 4);
   w.active = take((experts + 1) * 4);
   w.offset = take((experts + 1) * 4);
   w.token = take(pairs * 4);
   w.weight = take(pairs * 4);
-  w.inner = take(pairs * mx_blocks(i) * MX_BLOCK * 2 * (kind == F16 ? 2 : 1));
+  w.inner = take(pairs * mx_blocks(i) * MX_BLOCK * 4);
+  w.partial = take(w.parts * t * h * 4);
   return w;
 }
 
@@ -345,18 +433,28 @@ template <int KIND>
 static int launch_moe(const uint16_t* x, const uint16_t* router, const uint8_t* gate_up, const uint8_t* gate_up_scales,
                       const uint8_t* down, const uint8_t* down_scales, uint16_t* y, int t, int64_t h, int i, int experts,
                       int top_k, uint8_t* ws, hipStream_t stream) {
-  const Layout w = layout_of(KIND, t, h, i, experts, top_k);
+  const Layout w = layout_of(t, h, i, experts, top_k);
   const Routing route{(int*)(ws + w.active), (int*)(ws + w.offset), (int*)(ws + w.token), (float*)(ws + w.weight)};
-  float* partial = (float*)(ws + w.partial);
+  float* logits = (float*)(ws + w.logits);
   uint16_t* inner = (uint16_t*)(ws + w.inner);
   const int pairs = t * top_k, most = pairs < experts ? pairs : experts;
-  hipLaunchKernelGGL((moe_logits<KIND>), dim3((unsigned)((experts + 15) / 16), (unsigned)((t + 15) / 16), (unsigned)w.parts),
-                     dim3(256), 0, stream, x, router, partial, t, h, experts, w.steps);
-  hipLaunchKernelGGL(moe_route, dim3(1), dim3(1024), 0, stream, partial, w.parts, t, experts, top_k, route);
-  hipLaunchKernelGGL((moe_up<KIND>), dim3((unsigned)(mx_blocks(i) * 2), (unsigned)most), dim3(256), 0, stream, x, gate_up,
-                     gate_up_scales, inner, route, h, i, pairs);
-  hipLaunchKernelGGL((moe_down<KIND>), dim3((unsigned)((h + 15) / 16)), dim3(512), 0, stream, inner, down, down_scales, y, route,
-                     t, h, i, pairs);
+  const int64_t slabs = (mx_blocks(h) + SLAB - 1) / SLAB;
+  const int rows = t < 16 ? t : 16;
+  // as many waves to a row's slabs as its tokens leave LDS for two workgroups on a CU, and no more than there are slabs
+  int kparts = 8;
+  while (kparts > 1 && (kparts > slabs || kparts * rows * STAGED_ROW * (KIND == F16 ? 2 : 1) > 64 * 1024)) kparts /= 2;
+  hipLaunchKernelGGL((moe_logits<KIND>), dim3((unsigned)((experts + 15) / 16), (unsigned)((t + 15) / 16), PARTS), dim3(256), 0,
+                     stream, x, router, logits, t, h, experts);
+  auto choose = experts <= 64 ? moe_route<1> : experts <= 256 ? moe_route<4> : moe_route<16>;
+  hipLaunchKernelGGL(choose, dim3(1), dim3(1024), 0, stream, logits, t, experts, top_k, route);
+  hipLaunchKernelGGL((moe_up<KIND>), dim3((unsigned)((mx_blocks(i) * 2 * kparts + 7) / 8), (unsigned)most), dim3(512),
+                     (unsigned)(kparts * rows * STAGED_ROW * (KIND == F16 ? 2 : 1)), stream, x, gate_up, gate_up_scales, inner,
+                     route, h, i, pairs, kparts, rows);
+  float* partial = (float*)(ws + w.partial);
+  hipLaunchKernelGGL(moe_down, dim3((unsigned)((h + 255) / 256), (unsigned)w.parts), dim3(512),
+                     (unsigned)(4 * rows * STAGED_ROW + t * 1024), stream, inner, down, down_scales, partial, route, t, h, i, pairs,
+                     rows);
+  hipLaunchKernelGGL((moe_sum<KIND>), dim3((unsigned)((t * h + 255) / 256)), dim3(256), 0, stream, partial, y, t * h, w.parts);
   const hipError_t err = hipGetLastError();
   if (err == hipSuccess) return 0;
   krn_set_error("moe launch: %s", hipGetErrorString(err));
@@ -367,7 +465,7 @@ extern "C" {
 
 // See include/krn_amd.h for the contract of each entry point.
 int64_t krn_moe_workspace(int kind, int64_t t, int64_t h, int64_t i, int64_t experts, int64_t top_k) {
-  return moe_sizes(t, h, i, experts, top_k) && t > 0 ? layout_of(kind, t, h, i, experts, top_k).bytes : 0;
+  return moe_sizes(t, h, i, experts, top_k) && t > 0 ? layout_of(t, h, i, experts, top_k).bytes : 0;
 }
 
 int krn_moe(int kind, const void* x, const void* router, const void* gate_up, const void* gate_up_scales, const void* down,
@@ -388,7 +486,7 @@ int krn_moe(int kind, const void* x, const void* router, const void* gate_up, co
     krn_set_error("moe: codes and workspace start at 16-byte aligned addresses");
     return -1;
   }
-  const Layout w = layout_of(kind, t, h, i, experts, top_k);
+  const Layout w = layout_of(t, h, i, experts, top_k);
   if (workspace == nullptr || workspace_bytes < w.bytes) {
     krn_set_error("moe: a workspace of %lld bytes is needed", (long long)w.bytes);
     return -1;

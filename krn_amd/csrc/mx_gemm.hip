@@ -2,7 +2,6 @@
 // (the format and the order in which K is taken: mx_parts.h). v_mfma_scale_f32_16x16x128_f8f6f4 multiplies the codes and
 // applies both blocks' scales, so the operands stay in 4 bits until the matrix core; sums are float32 and every result is
 // rounded once. Every kernel computes blocks transposed (B A^T), so that a lane holds four neighbouring columns of one row.
-#include <stdlib.h>
 #include "gemm_split.h"
 #include "mx_parts.h"
 
@@ -257,17 +256,18 @@ __global__ __launch_bounds__(256) void mx_tile(const uint8_t* __restrict__ A, co
   _Pragma("unroll") for (int i = 0; i < TM * TN; ++i) {                                                                 \
     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                                                                  \
     if (i < TM + TN) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                                                 \
-    if (i >= TM * TN - LOADS_) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);                                       \
+    if (i >= TM * TN - (LOADS_)) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);                                       \
   }
 #define KRN_SLICE(kt, J0, J1, q)                                                                                        \
   do {                                                                                                                  \
     KRN_READ(1, kt, 1);                                                                                                 \
     issue_a((kt) + STAGES - 1);                                                                                         \
+    if (STAGES == 2) issue_b((kt) + 1); /* two stages: the next slice whole, to land by the barrier */                  \
     KRN_MMA(0, J0, q);                                                                                                  \
-    KRN_SPREAD(TM);                                                                                                     \
-    KRN_PUBLISH((STAGES - 3) * LOADS + TM);                                                                             \
+    KRN_SPREAD(STAGES == 2 ? TM + TN : TM);                                                                             \
+    KRN_PUBLISH(STAGES == 2 ? 0 : (STAGES - 3) * LOADS + TM);                                                           \
     KRN_READ(0, (kt) + 1, 0);                                                                                           \
-    issue_b((kt) + STAGES - 1);                                                                                         \
+    if (STAGES > 2) issue_b((kt) + STAGES - 1);                                                                         \
     KRN_MMA(1, J1, q);                                                                                                  \
     KRN_SPREAD(TN);                                                                                                     \
     __builtin_amdgcn_sched_barrier(0);                                                                                  \
@@ -586,39 +586,66 @@ static bool mx_epilogue(Epilogue& e, int out_kind, int nops, const int* ops, con
   return epilogue_of(e, out_kind, nops, ops, scalars, vectors, "mx_gemm");
 }
 
+// Few rows: 16 x (16 NT) columns a workgroup; then tiles, by their stages; then the four-wave loop on 256 x 256 tiles
+enum MxShape : int { FEW_16x16, FEW_16x32, FEW_16x64, FEW_32x16, FEW_32x32, TILE_64_SHORT, TILE_64, TILE_64_DEEP, TILE_64x128, TILE_128, QUAD };
 struct MxPlan {
-  int shape, parts;  // shape: 16-row blocks of the few-row kernel, or 100 + the tile
+  int shape, parts;
   int64_t workspace;
 };
 
-static MxPlan mx_plan(int64_t m, int64_t n, int64_t nb, int64_t workspace) {
-  const int force_shape = getenv("MX_SHAPE") ? atoi(getenv("MX_SHAPE")) : -1, force_parts = getenv("MX_PARTS") ? atoi(getenv("MX_PARTS")) : 1;
-  if (force_shape >= 0) return {force_shape, force_parts, force_parts > 1 ? force_parts * split_plane(m, n) : 0};
-  if (m <= 64) return {m <= 16 ? 0 : m <= 32 ? 1 : 2, 1, 0};
-  return {101, 1, 0};
+static MxPlan mx_plan(int64_t m, int64_t n, int64_t nb, bool activation, int64_t workspace) {
+  const int64_t slabs = (nb + SLAB - 1) / SLAB;
+  // Up to 32 rows: wider workgroups read A less often, narrower ones fill the chip (us, on 16 / 32 / 64 columns): 1 x 8192 x
+  // 8192 8.7 / 8.3 / 12.4, 16 x 14336 x 4096 11.3 / 9.3 / 8.7, 8 x 28672 x 8192 35.8 / 32.2 / 31.5; 24 x 4096 x 4096 5.5 /
+  // 6.9, 32 x 8192 x 8192 15.9 / 11.7, tiles of 64 x 64 7.7 and 11.9.
+  if (m <= 16) return {n >= 64 * 224 ? FEW_16x64 : n >= 32 * 256 ? FEW_16x32 : FEW_16x16, 1, 0};
+  if (m <= 32) return {n >= 32 * 256 ? FEW_32x32 : FEW_32x16, 1, 0};
+  // Estimated microseconds beyond a launch: what a slab takes the CU that holds most workgroups, measured at K = 8192
+  // (64 x 64 tiles, 256 workgroups 14.1 us, 512 21.8, 1024 39.1; eight stages 13.5, 24.5; 64 x 128 17.2, 35.3; 128 x 128 22.4,
+  // 52.3; 256 x 256 tiles, 128 of them 52.6, 256 66.3), and what parts add: their planes' way to the second launch and back
+  auto rounds = [&](int bm, int bn, int parts) {
+    return (double)((((m + bm - 1) / bm) * ((n + bn - 1) / bn) * parts + 255) / 256);
+  };
+  MxPlan best{TILE_64, 1, 0};
+  double least = 1e30;
+  for (int shape = TILE_64_SHORT; shape <= QUAD; ++shape)
+    for (int parts = 1; parts <= (shape == QUAD || shape == TILE_64_SHORT ? 1 : 8) && (parts == 1 || slabs / parts >= 2); ++parts) {
+      if (shape == QUAD && nb < SLAB) break;  // its scale loads take 16 bytes of a row
+      const int bm = shape <= TILE_64x128 ? 64 : shape == TILE_128 ? 128 : 256, bn = shape <= TILE_64_DEEP ? 64 : shape <= TILE_128 ? 128 : 256;
+      const double r = rounds(bm, bn, parts);
+      double slab = shape == TILE_64_SHORT ? 0.57 * r + 0.2 : shape == TILE_64 ? (r > 1 ? 0.53 * r : 0.57)
+                  : shape == TILE_64_DEEP ? (r > 1 ? 0.62 * r : 0.52) : shape == TILE_64x128 ? 0.93 * r : shape == TILE_128 ? 1.45 * r
+                                          : 3.0 * r + (rounds(256, 128, 1) > r ? 0.8 * r : 0);
+      // two stages let three workgroups share a CU and hide each other's first loads and stores, which is what a short K
+      // is made of (1000 x 3001 x 777, bias and gelu: 22.2 us with four, 17.4)
+      double us = (double)((slabs + parts - 1) / parts) * slab + (shape == TILE_64_SHORT ? 1.5 : 3.0) * r;
+      const int64_t need = parts > 1 ? parts * split_plane(m, n) : 0;
+      // an activation takes a CU's waves a time of its own for each 32 x 32 block they store, less where workgroups share it
+      if (activation && parts == 1)
+        us += r * (shape == TILE_64_SHORT ? 2.2 : shape == TILE_64 ? 2.7 : 4.8 * (bm / 64) * (bn / 64));
+      if (parts > 1) us += 4.0 + (double)need / 5e6;
+      if (need <= workspace && us < least) best = {shape, parts, need}, least = us;
+    }
+  return best;
 }
 
 static int launch_planned(const MxPlan& p, const MxCall& g) {
   switch (p.shape) {
-    case 0: return launch_few<1, 1, 4>(g);
-    case 1: return launch_few<2, 1, 4>(g);
-    case 2: return launch_few<4, 1, 4>(g);
-    case 3: return launch_few<1, 1, 8>(g);
-    case 4: return launch_few<1, 2, 4>(g);
-    case 5: return launch_few<1, 2, 8>(g);
-    case 6: return launch_few<1, 1, 16>(g);
-    case 100: return launch_tile<2, 2, 4>(g, p.parts);
-    case 101: return launch_tile<4, 4, 4>(g, p.parts);
-    case 200: {
-      if (g.nb < SLAB) return launch_tile<4, 4, 4>(g, p.parts);  // its scale loads take 16 bytes of a row
-      const dim3 tiles((unsigned)(((g.m + 255) / 256) * ((g.n + 255) / 256)));
-      if (g.nb % SLAB == 0) hipLaunchKernelGGL(mx_quad<false>, tiles, dim3(256), 0, g.stream, g.a, g.as, g.b, g.bs, g.c, g.m, g.n, g.nb, g.n, g.e);
-      else hipLaunchKernelGGL(mx_quad<true>, tiles, dim3(256), 0, g.stream, g.a, g.as, g.b, g.bs, g.c, g.m, g.n, g.nb, g.n, g.e);
-      return launched("mx_gemm");
-    }
-    case 103: return launch_tile<2, 4, 4>(g, p.parts);
-    default: return launch_tile<4, 2, 4>(g, p.parts);
+    case FEW_16x16: return launch_few<1, 1, 8>(g);
+    case FEW_16x32: return launch_few<1, 2, 8>(g);
+    case FEW_16x64: return launch_few<1, 4, 4>(g);
+    case FEW_32x16: return launch_few<2, 1, 4>(g);
+    case FEW_32x32: return launch_few<2, 2, 8>(g);
+    case TILE_64_SHORT: return launch_tile<2, 2, 2>(g, p.parts);
+    case TILE_64: return launch_tile<2, 2, 4>(g, p.parts);
+    case TILE_64_DEEP: return launch_tile<2, 2, 8>(g, p.parts);
+    case TILE_64x128: return launch_tile<2, 4, 4>(g, p.parts);
+    case TILE_128: return launch_tile<4, 4, 4>(g, p.parts);
   }
+  const dim3 tiles((unsigned)(((g.m + 255) / 256) * ((g.n + 255) / 256)));
+  auto kernel = g.nb % SLAB == 0 ? mx_quad<false> : mx_quad<true>;
+  hipLaunchKernelGGL(kernel, tiles, dim3(256), 0, g.stream, g.a, g.as, g.b, g.bs, g.c, g.m, g.n, g.nb, g.n, g.e);
+  return launched("mx_gemm");
 }
 
 extern "C" {
@@ -648,11 +675,15 @@ int krn_mx_gemm(const void* a, const void* a_scales, const void* b, const void* 
   }
   g.a = (const uint8_t*)a, g.as = (const uint8_t*)a_scales, g.b = (const uint8_t*)b, g.bs = (const uint8_t*)b_scales;
   g.c = c, g.m = m, g.n = n, g.nb = (int)nb, g.workspace = workspace, g.stream = (hipStream_t)stream;
-  return launch_planned(mx_plan(m, n, nb, workspace ? workspace_bytes : 0), g);
+  bool activation = false;
+  for (int i = 0; i < nops; ++i) activation |= (ops[i] & ((1 << VEC_KIND_SHIFT) - 1)) >= RELU;
+  return launch_planned(mx_plan(m, n, nb, activation, workspace ? workspace_bytes : 0), g);
 }
 
 int64_t krn_mx_gemm_workspace(int64_t m, int64_t n, int64_t k) {
-  return m <= 0 || n <= 0 || k <= 0 ? 0 : mx_plan(m, n, mx_blocks(k), INT64_MAX).workspace;
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  const int64_t plain = mx_plan(m, n, mx_blocks(k), false, INT64_MAX).workspace, with = mx_plan(m, n, mx_blocks(k), true, INT64_MAX).workspace;
+  return plain > with ? plain : with;
 }
 
 }  // extern "C"
