@@ -3,12 +3,16 @@
 // w_t the softmax of the chosen experts' router logits x_t . router_e. Ties go to the expert of the lower index; a NaN logit
 // counts as the largest.
 //
-// Bound by reading the chosen experts' weights, each once whatever the number of its tokens (up to 16). Four launches:
-//   logits  x router^T in 16-bit MFMAs (products exact, float32 sums)
+// Bound by reading the chosen experts' weights, each once whatever the number of its tokens (up to 16). The launches:
+//   logits  x router^T in 16-bit MFMAs (products exact, float32 sums), in parts of K
 //   route   one workgroup: a wave chooses a token's experts; every expert's tokens as a 64-bit mask, so that its count and a
 //           token's place in it are population counts and no order of atomics shows; the chosen experts in a row
 //   up      16 inner values of a chosen expert a wave: gate and up rows, w silu(gate) up to memory
-//   down    a workgroup per 16 outputs: all chosen experts' rows, added per token
+//   down    256 outputs a workgroup: all chosen experts' rows, added per token, in parts
+//   sum     the parts, in their order
+// Up to 8 tokens, which wait for launches more than for memory, have no second one: every workgroup of `up` routes for
+// itself (1 token: 14.4 + 3.5 us -> 13.0). The sum stays a launch of its own (2.6 us): with the last workgroup at its
+// outputs adding the parts up, the fence between them took `down` from 8 us to 18.
 // Weights go to bf16 exactly (v_cvt_scalef32_pk_bf16_fp4: two bits of mantissa and a power of two) and are multiplied in
 // 16x16x32 bf16 MFMAs, 16 weight rows by up to 16 tokens. bfloat16 tokens are taken as they are; float16 tokens are split
 // into the nearest bf16 and the bf16 of what is left, which holds all of a float16. The inner values are handed on as two
@@ -100,7 +104,46 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// EPL: experts a lane
+// The experts of token t, by one wave: lane j < top_k gets choice j and its weight. EPL: experts a lane
+template <int EPL>
+__device__ __forceinline__ void choose(const float* __restrict__ partial, int t, int T, int E, int top_k, int lane, int& pick,
+                                       float& weight) {
+  uint32_t key[EPL];  // expert lane + 64 i, 0 once chosen and past the last
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    const int e = lane + 64 * i;
+    float v[PARTS];
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) v[p] = partial[((int64_t)p * T + t) * E + min(e, E - 1)];
+    float sum = v[0];
+#pragma unroll
+    for (int p = 1; p < PARTS; ++p) sum += v[p];
+    key[i] = e < E ? ordered(sum) : 0;
+    if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // 32 loads at a time: all of them do not fit the registers
+  }
+  float mine = -INFINITY;  // lane j: the logit of choice j
+  pick = 0;
+  for (int j = 0; j < top_k; ++j) {
+    uint32_t best = key[0];
+#pragma unroll
+    for (int i = 1; i < EPL; ++i) best = max(best, key[i]);
+    best = wave_extreme<true>(best);
+    uint32_t e = MOE_EXPERTS;  // the lowest expert with that logit
+#pragma unroll
+    for (int i = EPL - 1; i >= 0; --i) e = key[i] == best ? lane + 64 * i : e;
+    e = wave_extreme<false>(e);
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) key[i] = lane + 64 * i == (int)e ? 0 : key[i];
+    if (lane == j) mine = __uint_as_float(best & 0x80000000u ? best ^ 0x80000000u : ~best), pick = (int)e;
+  }
+  const float top = __shfl(mine, 0);
+  const float p = lane < top_k ? expf(mine - top) : 0.0f;
+  float sum = p;
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) sum += __shfl_xor(sum, d);
+  weight = p / sum;
+}
+
 template <int EPL>
 __global__ __launch_bounds__(1024) void moe_route(const float* __restrict__ partial, int T, int E, int top_k, Routing out) {
   __shared__ unsigned long long mask[MOE_EXPERTS];
@@ -111,41 +154,11 @@ __global__ __launch_bounds__(1024) void moe_route(const float* __restrict__ part
   mask[threadIdx.x] = 0;
   __syncthreads();
   for (int t = wave; t < T; t += 16) {
-    uint32_t key[EPL];  // expert lane + 64 i, 0 once chosen and past the last
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      const int e = lane + 64 * i;
-      float v[PARTS];
-#pragma unroll
-      for (int p = 0; p < PARTS; ++p) v[p] = partial[((int64_t)p * T + t) * E + min(e, E - 1)];
-      float sum = v[0];
-#pragma unroll
-      for (int p = 1; p < PARTS; ++p) sum += v[p];
-      key[i] = e < E ? ordered(sum) : 0;
-    }
-    float mine = -INFINITY;  // lane j: the logit of choice j
-    int pick = 0;
-    for (int j = 0; j < top_k; ++j) {
-      uint32_t best = key[0];
-#pragma unroll
-      for (int i = 1; i < EPL; ++i) best = max(best, key[i]);
-      best = wave_extreme<true>(best);
-      uint32_t e = MOE_EXPERTS;  // the lowest expert with that logit
-#pragma unroll
-      for (int i = EPL - 1; i >= 0; --i) e = key[i] == best ? lane + 64 * i : e;
-      e = wave_extreme<false>(e);
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) key[i] = lane + 64 * i == (int)e ? 0 : key[i];
-      if (lane == j) mine = __uint_as_float(best & 0x80000000u ? best ^ 0x80000000u : ~best), pick = (int)e;
-    }
-    const float top = __shfl(mine, 0);
-    const float p = lane < top_k ? expf(mine - top) : 0.0f;
-    float sum = p;
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2) sum += __shfl_xor(sum, d);
+    int pick;
+    float w;
+    choose<EPL>(partial, t, T, E, top_k, lane, pick, w);
     if (lane < top_k) {
-      chosen[t * top_k + lane] = pick;
-      weight[t * top_k + lane] = p / sum;
+      chosen[t * top_k + lane] = pick, weight[t * top_k + lane] = w;
       atomicOr(&mask[pick], 1ull << t);
     }
   }
@@ -175,6 +188,46 @@ __global__ __launch_bounds__(1024) void moe_route(const float* __restrict__ part
     const int at = (int)base[expert] + __popcll(mask[expert] & ((1ull << t) - 1));
     out.token[at] = t, out.weight[at] = weight[i];
   }
+}
+
+// The routing of up to FEW tokens by one workgroup, in its LDS: a pair (token, choice) finds its place by counting the pairs of
+// lower experts and the earlier ones of its own
+constexpr int FEW = 8, FEW_PAIRS = FEW * MOE_TOP_K;
+struct FewRouting {
+  int active[FEW_PAIRS + 1], offset[FEW_PAIRS + 1], token[FEW_PAIRS], chosen[FEW_PAIRS];
+  float weight[FEW_PAIRS], given[FEW_PAIRS];
+  bool first[FEW_PAIRS];
+};
+
+template <int EPL>
+__device__ __forceinline__ void route_few(FewRouting& out, const float* __restrict__ partial, int T, int E, int top_k) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = threadIdx.x, pairs = T * top_k;
+  if (wave < T) {
+    int pick;
+    float w;
+    choose<EPL>(partial, wave, T, E, top_k, lane, pick, w);
+    if (lane < top_k) out.chosen[wave * top_k + lane] = pick, out.given[wave * top_k + lane] = w;
+  }
+  __syncthreads();
+  int below = 0, before = 0;
+  const int e = i < pairs ? out.chosen[i] : 0;
+  if (i < pairs) {
+    for (int j = 0; j < pairs; ++j) below += out.chosen[j] < e, before += j < i && out.chosen[j] == e;
+    out.first[i] = before == 0;
+    out.token[below + before] = i / top_k, out.weight[below + before] = out.given[i];
+  }
+  __syncthreads();
+  if (i < pairs && before == 0) {
+    int rank = 0;
+    for (int j = 0; j < pairs; ++j) rank += out.first[j] && out.chosen[j] < e;
+    out.active[1 + rank] = e, out.offset[rank] = below;
+  }
+  if (i == 0) {
+    int active = 0;
+    for (int j = 0; j < pairs; ++j) active += out.first[j];
+    out.active[0] = active, out.offset[active] = pairs;
+  }
+  __syncthreads();
 }
 
 // Eight codes of a block as bf16 values
@@ -230,13 +283,26 @@ __device__ __forceinline__ u32x4 staged(const uint8_t* slab, int row, int j, int
 // Inner values of the chosen expert blockIdx.y for its tokens, `rows` (at most 16) at a time. Eight waves: `kparts` of them
 // split the slabs of 16 gate and 16 up rows, so that a workgroup has 8 / kparts times 16 inner values. Past the
 // inner size, up to whole blocks, zeros. Dynamic LDS: kparts slabs of `rows` tokens (float16: of both parts).
-template <int KIND>
+// EPL > 0: of up to FEW tokens, whose routing the workgroup does itself, the first one for `down` as well.
+template <int KIND, int EPL>
 __global__ __launch_bounds__(512) void moe_up(const uint16_t* __restrict__ X, const uint8_t* __restrict__ W,
-                                              const uint8_t* __restrict__ S, uint16_t* __restrict__ inner, Routing route,
-                                              int64_t H, int I, int pairs, int kparts, int rows) {
+                                              const uint8_t* __restrict__ S, uint16_t* __restrict__ inner, Routing given,
+                                              int64_t H, int I, int pairs, int kparts, int rows,
+                                              const float* __restrict__ partial, int T, int E, int top_k) {
   constexpr int PLANES = KIND == F16 ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) uint8_t tokens[];
   __shared__ f32x4 sums[8][2][64];
+  __shared__ FewRouting few;
+  Routing route = given;
+  if constexpr (EPL > 0) {
+    route_few<EPL>(few, partial, T, E, top_k);
+    route = Routing{few.active, few.offset, few.token, few.weight};
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x <= pairs) {
+      const int i = threadIdx.x, active = few.active[0];
+      if (i <= active) given.active[i] = few.active[i], given.offset[i] = few.offset[i];
+      if (i < pairs) given.token[i] = few.token[i], given.weight[i] = few.weight[i];
+    }
+  }
   const int a = blockIdx.y;
   if (a >= route.active[0]) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
@@ -285,6 +351,7 @@ __global__ __launch_bounds__(512) void moe_up(const uint16_t* __restrict__ X, co
             gate = mfma16<BF16>(gv, v, gate), up = mfma16<BF16>(uv, v, up);
           }
         }
+        __builtin_amdgcn_sched_barrier(0);  // operands of one step at a time in registers, not of all four
       }
     }
     sums[wave][0][lane] = gate, sums[wave][1][lane] = up;
@@ -306,9 +373,10 @@ __global__ __launch_bounds__(512) void moe_up(const uint16_t* __restrict__ X, co
 }
 
 // Outputs n0 .. n0 + 255 of every token over part blockIdx.y of the chosen experts' slabs: each of the eight waves has 32
-// weight rows and goes through all of the part, its next slab's weights on their way; the waves share the inner values in
-// LDS, two slabs' places in turn. An expert's part goes to its tokens' sums, which only the wave with those rows touches.
-// Dynamic LDS: two slabs of `rows` tokens (at most 16) in two parts, then the sums of T tokens.
+// weight rows and goes through all of the part. The waves share the tokens' inner values in LDS, `rows` tokens (at
+// most 16) a step, in two places in turn; a step's inner values and a slab's weights are on their way while the step
+// before is multiplied. An expert's part goes to its tokens' sums, which only the wave with those rows touches.
+// Dynamic LDS: two places of `rows` tokens in two parts, then the sums of T tokens.
 __global__ __launch_bounds__(512) void moe_down(const uint16_t* __restrict__ inner, const uint8_t* __restrict__ W,
                                                 const uint8_t* __restrict__ S, float* __restrict__ partial, Routing route,
                                                 int T, int64_t H, int I, int pairs, int rows) {
@@ -321,33 +389,59 @@ __global__ __launch_bounds__(512) void moe_down(const uint16_t* __restrict__ inn
   const int nb = (int)mx_blocks(I), slabs = (nb + SLAB - 1) / SLAB, items = route.active[0] * slabs;
   const int64_t pitch = (int64_t)nb * MX_BLOCK;
   const int first = (int)((int64_t)items * blockIdx.y / gridDim.y), end = (int)((int64_t)items * (blockIdx.y + 1) / gridDim.y);
-  auto load = [&](WeightSlab (&w)[2], int item) {
-    const int a = item / slabs;
-    const int64_t expert = route.active[1 + a] * H;
+  struct Step {  // tokens f .. of the expert of item `item`, `begin` .. `begin + count` among the pairs
+    int item, slab, f, begin, count, expert;
+  };
+  auto at_item = [&](int item) {
+    const int a = item / slabs, begin = route.offset[a];
+    return Step{item, item - a * slabs, 0, begin, route.offset[a + 1] - begin, route.active[1 + a]};
+  };
+  auto load = [&](WeightSlab (&w)[2], const Step& s) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int64_t at = (expert + min(n0 + 16 * i + r, H - 1)) * nb;
-      w[i].load(W + at * 16, S + at, item - a * slabs, nb, g);
+      const int64_t at = ((int64_t)s.expert * H + min(n0 + 16 * i + r, H - 1)) * nb;
+      w[i].load(W + at * 16, S + at, s.slab, nb, g);
     }
   };
-  WeightSlab now[2];
-  if (first < end) load(now, first);
-  int place = 0;
-  for (int item = first; item < end; ++item) {
-    WeightSlab next[2] = {now[0], now[1]};
-    if (item + 1 < end) load(next, item + 1);
-    const int a = item / slabs, s = item - a * slabs, begin = route.offset[a], count = route.offset[a + 1] - begin;
-    for (int f = 0; f < count; f += rows) {
-      const int here = min(count - f, rows), own = min(r, here - 1);
-      uint8_t* at = tokens + place * 2 * plane;
-      place ^= 1;
-      for (int i = wave; i < 2 * here; i += 8) {
-        const int t = i >> 1, block = slab_block(s, nb) + (lane >> 2);
-        const uint16_t* from = inner + ((i & 1) * pairs + begin + f + t) * pitch + (int64_t)block * 32 + 8 * (lane & 3);
-        *reinterpret_cast<u32x4*>(at + (i & 1) * plane + t * STAGED_ROW + lane * 16) =
-            in_slab(block, s, nb) ? *reinterpret_cast<const u32x4*>(from) : u32x4{};
-      }
-      __syncthreads();  // and every wave is done with what was in this place two slabs ago
+  // row i of a step: token i / 2, part i % 2; this wave's rows are wave, wave + 8, ...
+  auto fetch = [&](u32x4 (&v)[4], const Step& s) {
+    const int block = slab_block(s.slab, nb) + (lane >> 2), here = min(s.count - s.f, rows);
+    const bool in = in_slab(block, s.slab, nb);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = wave + 8 * k;
+      v[k] = u32x4{};
+      if (i < 2 * here && in)
+        v[k] = *reinterpret_cast<const u32x4*>(inner + ((i & 1) * pairs + s.begin + s.f + (i >> 1)) * pitch +
+                                               (int64_t)block * 32 + 8 * (lane & 3));
+    }
+  };
+  auto put = [&](const u32x4 (&v)[4], uint8_t* place, const Step& s) {
+    const int here = min(s.count - s.f, rows);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = wave + 8 * k;
+      if (i < 2 * here) *reinterpret_cast<u32x4*>(place + (i & 1) * plane + (i >> 1) * STAGED_ROW + lane * 16) = v[k];
+    }
+  };
+  if (first < end) {
+    Step step = at_item(first);
+    WeightSlab now[2];
+    u32x4 v[4];
+    load(now, step);
+    fetch(v, step);
+    put(v, tokens, step);
+    for (int place = 0;; place ^= 1) {
+      __syncthreads();  // the step's values are there, and every wave is done with the other place
+      Step next = step;
+      next.f += rows;
+      const bool new_item = next.f >= step.count, more = !new_item || step.item + 1 < end;
+      if (new_item) next = at_item(min(step.item + 1, end - 1));
+      WeightSlab after[2];
+      load(after, next);  // the same again within an item: from the cache, and no branch around loads in flight
+      if (more) fetch(v, next);
+      const uint8_t* at = tokens + place * 2 * plane;
+      const int here = min(step.count - step.f, rows), own = min(r, here - 1);
       f32x4 acc[2] = {};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -357,17 +451,21 @@ __global__ __launch_bounds__(512) void moe_down(const uint16_t* __restrict__ inn
           const u32x4 v0 = bf16_codes(now[0].code[j][q], f0), v1 = bf16_codes(now[1].code[j][q], f1);
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
-            const u32x4 v = staged(at + p * plane, own, j, q, g);
-            acc[0] = mfma16<BF16>(v0, v, acc[0]), acc[1] = mfma16<BF16>(v1, v, acc[1]);
+            const u32x4 x = staged(at + p * plane, own, j, q, g);
+            acc[0] = mfma16<BF16>(v0, x, acc[0]), acc[1] = mfma16<BF16>(v1, x, acc[1]);
           }
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
       if (r < here) {
-        f32x4* sum = sums + route.token[begin + f + r] * 64 + g;
+        f32x4* sum = sums + route.token[step.begin + step.f + r] * 64 + g;
         sum[0] += acc[0], sum[4] += acc[1];
       }
+      if (!more) break;
+      put(v, tokens + (place ^ 1) * 2 * plane, next);
+      now[0] = after[0], now[1] = after[1];
+      step = next;
     }
-    now[0] = next[0], now[1] = next[1];
   }
   for (int i = lane; i < T * 8; i += 64) {
     const int t = i >> 3;
@@ -439,18 +537,25 @@ static int launch_moe(const uint16_t* x, const uint16_t* router, const uint8_t* 
   uint16_t* inner = (uint16_t*)(ws + w.inner);
   const int pairs = t * top_k, most = pairs < experts ? pairs : experts;
   const int64_t slabs = (mx_blocks(h) + SLAB - 1) / SLAB;
-  const int rows = t < 16 ? t : 16;
-  // as many waves to a row's slabs as its tokens leave LDS for two workgroups on a CU, and no more than there are slabs
+  float* partial = (float*)(ws + w.partial);
+  const bool few = t <= FEW;
+  // tokens gone through at a time: room for twice an expert's average, so that few experts are read twice for the rest
+  int rows = 4;
+  while (rows < 16 && rows < t && rows * experts < 2 * pairs) rows *= 2;
+  rows = rows < t ? rows : t;
+  // as many waves to a row's slabs as these leave LDS for two workgroups on a CU, and no more than there are slabs
   int kparts = 8;
-  while (kparts > 1 && (kparts > slabs || kparts * rows * STAGED_ROW * (KIND == F16 ? 2 : 1) > 64 * 1024)) kparts /= 2;
+  while (kparts > 1 && (kparts > slabs || kparts * rows * STAGED_ROW * (KIND == F16 ? 2 : 1) > 56 * 1024)) kparts /= 2;
   hipLaunchKernelGGL((moe_logits<KIND>), dim3((unsigned)((experts + 15) / 16), (unsigned)((t + 15) / 16), PARTS), dim3(256), 0,
                      stream, x, router, logits, t, h, experts);
-  auto choose = experts <= 64 ? moe_route<1> : experts <= 256 ? moe_route<4> : moe_route<16>;
-  hipLaunchKernelGGL(choose, dim3(1), dim3(1024), 0, stream, logits, t, experts, top_k, route);
-  hipLaunchKernelGGL((moe_up<KIND>), dim3((unsigned)((mx_blocks(i) * 2 * kparts + 7) / 8), (unsigned)most), dim3(512),
+  if (!few) {
+    auto choose = experts <= 64 ? moe_route<1> : experts <= 256 ? moe_route<4> : moe_route<16>;
+    hipLaunchKernelGGL(choose, dim3(1), dim3(1024), 0, stream, logits, t, experts, top_k, route);
+  }
+  auto up = !few ? moe_up<KIND, 0> : experts <= 64 ? moe_up<KIND, 1> : experts <= 256 ? moe_up<KIND, 4> : moe_up<KIND, 16>;
+  hipLaunchKernelGGL(up, dim3((unsigned)((mx_blocks(i) * 2 * kparts + 7) / 8), (unsigned)most), dim3(512),
                      (unsigned)(kparts * rows * STAGED_ROW * (KIND == F16 ? 2 : 1)), stream, x, gate_up, gate_up_scales, inner,
-                     route, h, i, pairs, kparts, rows);
-  float* partial = (float*)(ws + w.partial);
+                     route, h, i, pairs, kparts, rows, logits, t, experts, top_k);
   hipLaunchKernelGGL(moe_down, dim3((unsigned)((h + 255) / 256), (unsigned)w.parts), dim3(512),
                      (unsigned)(4 * rows * STAGED_ROW + t * 1024), stream, inner, down, down_scales, partial, route, t, h, i, pairs,
                      rows);

@@ -22,7 +22,7 @@ __host__ __device__ inline int64_t mx_blocks(int64_t k) { return (k + MX_BLOCK -
 // A row whose end cuts its last slab has that slab taken from its last 16 blocks: those of them that the slab before holds
 // already count as zeros there (the callers give their codes so), and the scales are 16 bytes of the row as they lie. (A
 // scale of 255 among the blocks taken twice makes both products NaN, as one does.) A row of fewer than 16 blocks is
-// one slab; its scales go byte by byte, 2^0 past its end, so that no byte outside the row is read.
+// one slab; its scales go word by word, 2^0 past its end. No byte outside the row is read.
 __device__ __forceinline__ int slab_block(int slab, int nb) { return nb < SLAB ? 0 : min(slab * SLAB, nb - SLAB); }
 
 // Whether block `block` counts in slab `slab` of a row of `nb` blocks
@@ -33,14 +33,20 @@ __device__ __forceinline__ u32x4 long_scales(const uint8_t* row, int slab, int n
 }
 
 __device__ __forceinline__ u32x4 short_scales(const uint8_t* row, int nb) {  // nb < 16
-  uint32_t b[SLAB];
+  typedef uint32_t u32_any __attribute__((aligned(1)));
+  constexpr uint32_t UNIT = 0x7f7f7f7f;
+  u32x4 w = {UNIT, UNIT, UNIT, UNIT};
+  if (nb < 4) {
+    const uint32_t b0 = row[0], b1 = nb > 1 ? row[1] : 0x7f, b2 = nb > 2 ? row[2] : 0x7f;
+    w[0] = b0 | b1 << 8 | b2 << 16 | 0x7fu << 24;
+    return w;
+  }
 #pragma unroll
-  for (int i = 0; i < SLAB; ++i) b[i] = row[min(i, nb - 1)];
-#pragma unroll
-  for (int i = 0; i < SLAB; ++i) b[i] = i < nb ? b[i] : 0x7f;
-  u32x4 w;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = b[4 * i] | b[4 * i + 1] << 8 | b[4 * i + 2] << 16 | b[4 * i + 3] << 24;
+  for (int i = 0; i < 4; ++i) {  // the word that the row's end cuts is its last four bytes, shifted
+    const int at = min(4 * i, nb - 4), cut = 4 * i - at;
+    const uint32_t v = *reinterpret_cast<const u32_any*>(row + at);
+    w[i] = cut < 4 ? __builtin_amdgcn_alignbyte(UNIT, v, cut) : UNIT;
+  }
   return w;
 }
 
