@@ -568,13 +568,13 @@ __device__ __forceinline__ void patch_put_t(const V& block, uint32_t* patch, int
 // W8A8 M = 4096 0.272 -> 0.247 ms; write-back instead of non-temporal stores: bf16 1.5 % slower.
 template <bool INT, bool BF, typename V4, typename Ops>
 __device__ __forceinline__ void store16t_direct(const V4 (&acc)[8][8], Ops ops, void* C, int64_t ldc, int64_t row0,
-                                                int64_t col0, int lane) {
+                                                int64_t col0, int lane, int64_t rows = 128) {
   const int r16 = lane & 15, g = lane >> 4;
   const uint64_t base = (uint64_t)(static_cast<uint16_t*>(C) + row0 * ldc + col0);
   const uint32_t base_lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)base);
   const uint32_t base_hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(base >> 32));
   const void* region = (const void*)(((uint64_t)base_hi << 32) | (uint64_t)base_lo);
-  const __amdgpu_buffer_rsrc_t out = panel_rsrc(region, (int64_t)128 * ldc * 2);
+  const __amdgpu_buffer_rsrc_t out = panel_rsrc(region, rows * ldc * 2);  // stores to rows past `rows` do nothing
   // after the exchange below, lane group g holds the 16 columns of block 4 jj + g of its row: two 16-byte pieces
   const uint32_t lane_off = (uint32_t)((r16 * ldc + 16 * g) * 2);
 #pragma unroll

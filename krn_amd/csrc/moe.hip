@@ -10,8 +10,9 @@
 //   up      16 inner values of a chosen expert a wave: gate and up rows, w silu(gate) up to memory
 //   down    256 outputs a workgroup: all chosen experts' rows, added per token, in parts
 //   sum     the parts, in their order
-// Up to 8 tokens, which wait for launches more than for memory, have no second one: every workgroup of `up` routes for
-// itself (1 token: 14.4 + 3.5 us -> 13.0). The sum stays a launch of its own (2.6 us): with the last workgroup at its
+// One or two tokens, which wait for launches more than for memory, have no second one: every workgroup of `up` routes for
+// itself (of 64 experts 4096 x 2048, us: 1 token 28.6 -> 26.0, 2 tokens 45.0 -> 42.6; but 4 tokens 68.8 -> 73.1, where
+// more workgroups do it one after the other). The sum stays a launch of its own (2.6 us): with the last workgroup at its
 // outputs adding the parts up, the fence between them took `down` from 8 us to 18.
 // Weights go to bf16 exactly (v_cvt_scalef32_pk_bf16_fp4: two bits of mantissa and a power of two) and are multiplied in
 // 16x16x32 bf16 MFMAs, 16 weight rows by up to 16 tokens. bfloat16 tokens are taken as they are; float16 tokens are split
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(1024) void moe_route(const float* __restrict__ part
 
 // The routing of up to FEW tokens by one workgroup, in its LDS: a pair (token, choice) finds its place by counting the pairs of
 // lower experts and the earlier ones of its own
-constexpr int FEW = 8, FEW_PAIRS = FEW * MOE_TOP_K;
+constexpr int FEW = 2, FEW_PAIRS = FEW * MOE_TOP_K;
 struct FewRouting {
   int active[FEW_PAIRS + 1], offset[FEW_PAIRS + 1], token[FEW_PAIRS], chosen[FEW_PAIRS];
   float weight[FEW_PAIRS], given[FEW_PAIRS];

@@ -156,10 +156,82 @@ __device__ __forceinline__ void spread_scales(const u32x4& d, uint32_t (&out)[4]
 #pragma unroll
   for (int n = 0; n < 6; ++n) s.step(n, d, out);
 }
-// One 32 x 32 block from its patch to C, rows at any alignment. Out of line: each wave stores several blocks
-__device__ __noinline__ void patch_store_any(uint32_t* patch, void* C, int64_t ldc, int64_t row0, int64_t col0, int64_t M,
-                                             int64_t N, const Epilogue& e, int lane) {
-  patch_store_inline<false, true, false, true>(patch, C, ldc, row0, col0, M, N, e, lane);
+// One 32 x 32 block from its patch through the epilogue to C, rows at any alignment: lane l has columns 16 (l & 1) .. + 15 of
+// row l / 2. Out of line, each wave storing several blocks. What an operation does is decided once for all its
+// values, so that their chains of dependent instructions overlap, eight at a time (4096 x 14336 x 4096 with silu, decided value by
+// value as in the other formats' store: 566 us, 166 here).
+__device__ __noinline__ void store_patch(uint32_t* patch, void* C, int64_t ldc, int64_t row0, int64_t col0, int64_t M,
+                                         int64_t N, const Epilogue& e, int lane) {
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the patch is written before any lane reads it
+  __builtin_amdgcn_wave_barrier();
+  const int rr = lane >> 1, c0 = (lane & 1) * 16;
+  float v[16];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const f32x4 w = *reinterpret_cast<const f32x4*>(patch + rr * PATCH_STRIDE + c0 + 4 * q);
+    v[4 * q] = w[0], v[4 * q + 1] = w[1], v[4 * q + 2] = w[2], v[4 * q + 3] = w[3];
+  }
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  __builtin_amdgcn_wave_barrier();  // the next block may overwrite the patch
+  const int64_t m = row0 + rr, n = col0 + c0;
+  if (m >= M || n >= N) return;
+  const int cols = (int)min(N - n, (int64_t)16);
+  for (int i = 0; i < e.nops; ++i) {
+    const int op = e.op[i] & ((1 << VEC_KIND_SHIFT) - 1), kind = e.op[i] >> VEC_KIND_SHIFT;
+#define KRN_ALL(x)                                                       \
+  _Pragma("unroll") for (int half = 0; half < 16; half += 8) {             \
+    _Pragma("unroll") for (int c = half; c < half + 8; ++c) v[c] = x;      \
+    __builtin_amdgcn_sched_barrier(0); /* eight at a time: registers */    \
+  }
+    if (op == RELU) { KRN_ALL(activation(RELU, v[c])); }
+    else if (op == GELU) { KRN_ALL(activation(GELU, v[c])); }
+    else if (op == SILU) { KRN_ALL(activation(SILU, v[c])); }
+    else if (op % 3 == 2) {
+      float s[16];
+      if (kind == 0) {
+        const float* p = static_cast<const float*>(e.vec[i]) + n;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) s[c] = p[min(c, cols - 1)];
+      } else {
+        const uint16_t* p = static_cast<const uint16_t*>(e.vec[i]) + n;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) s[c] = bits_value(kind, p[min(c, cols - 1)]);
+      }
+      if (op == MUL_COL) { KRN_ALL(__fmul_rn(v[c], s[c])); }
+      else { KRN_ALL(__fadd_rn(v[c], s[c])); }
+    } else {
+      const float s = op % 3 == 0 ? e.scalar[i] : bits_value(kind, vec_bits(e.vec[i], kind, m));
+      if (op < 3) { KRN_ALL(__fmul_rn(v[c], s)); }
+      else { KRN_ALL(__fadd_rn(v[c], s)); }
+    }
+#undef KRN_ALL
+  }
+  if (e.out_kind == F32) {
+    float* out = static_cast<float*>(C) + m * ldc + n;
+    if (cols == 16) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        reinterpret_cast<u32x4_any*>(out)[q] = __builtin_bit_cast(u32x4, f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]});
+    } else {
+#pragma unroll
+      for (int c = 0; c < 16; ++c)
+        if (c < cols) out[c] = v[c];
+    }
+    return;
+  }
+  uint32_t h[8];
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    h[c] = e.out_kind == BF16 ? f2bf2(v[2 * c], v[2 * c + 1]) : (uint32_t)f2h(v[2 * c]) | (uint32_t)f2h(v[2 * c + 1]) << 16;
+  uint16_t* out = static_cast<uint16_t*>(C) + m * ldc + n;
+  if (cols == 16) {
+    reinterpret_cast<u32x4_any*>(out)[0] = u32x4{h[0], h[1], h[2], h[3]};
+    reinterpret_cast<u32x4_any*>(out)[1] = u32x4{h[4], h[5], h[6], h[7]};
+  } else {
+#pragma unroll
+    for (int c = 0; c < 16; ++c)
+      if (c < cols) out[c] = (uint16_t)(h[c >> 1] >> ((c & 1) * 16));
+  }
 }
 
 // Tiles of 32 TM x 32 TN, four waves of 16 TM x 16 TN each, K in `parts` runs of slabs (blockIdx.y). Slices of 128 bytes a
@@ -328,7 +400,7 @@ __global__ __launch_bounds__(256) void mx_tile(const uint8_t* __restrict__ A, co
 #pragma unroll
         for (int q = 0; q < 2; ++q)
           *reinterpret_cast<f32x4*>(patch + (16 * p + r) * PATCH_STRIDE + 16 * q + 4 * g) = acc[i + p][k + q];
-      patch_store_any(patch, C, ldc, m0 + wm * (16 * TM) + 16 * i, n0 + wn * (16 * TN) + 16 * k, M, N, local, lane);
+      store_patch(patch, C, ldc, m0 + wm * (16 * TM) + 16 * i, n0 + wn * (16 * TN) + 16 * k, M, N, local, lane);
     }
 }
 
@@ -349,8 +421,10 @@ __global__ __launch_bounds__(256) void mx_tile(const uint8_t* __restrict__ A, co
 // of half q / 2 of a 32-row block. The next two slabs' are loaded at the ends of the second and third slice, and spread
 // between the MFMAs of the fourth.
 //
-// CUT: rows end inside a slab. Rows hold a slab at least.
-template <bool CUT>
+// CUT: rows end inside a slab. Rows hold a slab at least. DIRECT: the epilogue and N are the direct
+// store's (quad16_direct), whose stores past the last row do nothing; otherwise all blocks go through patches. (Both
+// stores in one kernel leave the loop too few registers.)
+template <bool CUT, bool DIRECT>
 __global__ __launch_bounds__(256, 1) void mx_quad(const uint8_t* __restrict__ A, const uint8_t* __restrict__ AS,
                                                   const uint8_t* __restrict__ B, const uint8_t* __restrict__ BS,
                                                   void* __restrict__ C, int64_t M, int64_t N, int nb, int64_t ldc, Epilogue e) {
@@ -540,9 +614,28 @@ __global__ __launch_bounds__(256, 1) void mx_quad(const uint8_t* __restrict__ A,
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
   __syncthreads();
   const int64_t row0 = m0 + wm * 128, col0 = n0 + wn * 128;
+  if constexpr (DIRECT) {
+    if (row0 >= M || col0 >= N) return;  // N is a multiple of 128
+    const int64_t rows = min(M - row0, (int64_t)128);
+    Quad16Generic ops;
+    quad16_generic(ops, e, row0, col0, lane);
+    if (e.out_kind == BF16) store16t_direct<false, true>(acc, ops, C, ldc, row0, col0, lane, rows);
+    else store16t_direct<false, false>(acc, ops, C, ldc, row0, col0, lane, rows);
+    return;
+  }
   uint32_t* patch = reinterpret_cast<uint32_t*>(la0) + wave * PATCH_WORDS;
-  store_tile16t<false, f32x16>(acc, quad16_direct(e, C, ldc, row0, col0, M, N), false, Quad16RowCol{}, patch, C, ldc, row0,
-                               col0, M, N, e, lane);
+  const Epilogue local = e;  // taken by address by the out-of-line store
+#pragma unroll
+  for (int i = 0; i < 8; i += 2)
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          *reinterpret_cast<f32x4*>(patch + (16 * p + r16) * PATCH_STRIDE + 16 * q + 4 * g4) = agpr_block(acc[i + p][k + q]);
+      store_patch(patch, C, ldc, row0 + 16 * i, col0 + 16 * k, M, N, local, lane);
+    }
 }
 
 }  // namespace krn
@@ -622,7 +715,7 @@ static MxPlan mx_plan(int64_t m, int64_t n, int64_t nb, bool activation, int64_t
       const int64_t need = parts > 1 ? parts * split_plane(m, n) : 0;
       // an activation takes a CU's waves a time of its own for each 32 x 32 block they store, less where workgroups share it
       if (activation && parts == 1)
-        us += r * (shape == TILE_64_SHORT ? 2.2 : shape == TILE_64 ? 2.7 : 4.8 * (bm / 64) * (bn / 64));
+        us += r * (shape <= TILE_64 ? 1.6 : 2.2 * (bm / 64) * (bn / 64));
       if (parts > 1) us += 4.0 + (double)need / 5e6;
       if (need <= workspace && us < least) best = {shape, parts, need}, least = us;
     }
@@ -643,7 +736,14 @@ static int launch_planned(const MxPlan& p, const MxCall& g) {
     case TILE_128: return launch_tile<4, 4, 4>(g, p.parts);
   }
   const dim3 tiles((unsigned)(((g.m + 255) / 256) * ((g.n + 255) / 256)));
-  auto kernel = g.nb % SLAB == 0 ? mx_quad<false> : mx_quad<true>;
+  bool direct = (g.e.out_kind == BF16 || g.e.out_kind == F16) && g.e.nops <= DIRECT_OPS && g.n % 128 == 0 &&
+                (uintptr_t)g.c % 8 == 0 && 256 * g.n <= 0x7fffffff;
+  for (int i = 0; i < g.e.nops; ++i) {
+    const int op = g.e.op[i] & ((1 << VEC_KIND_SHIFT) - 1);
+    direct &= op < RELU && (op % 3 != 1 || g.m % 128 == 0);  // it reads a row vector for whole quarters
+  }
+  auto kernel = g.nb % SLAB == 0 ? (direct ? mx_quad<false, true> : mx_quad<false, false>)
+                                 : (direct ? mx_quad<true, true> : mx_quad<true, false>);
   hipLaunchKernelGGL(kernel, tiles, dim3(256), 0, g.stream, g.a, g.as, g.b, g.bs, g.c, g.m, g.n, g.nb, g.n, g.e);
   return launched("mx_gemm");
 }

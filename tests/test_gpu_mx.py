@@ -265,3 +265,24 @@ def test_submit_and_rebind(device):
     bound()
     np.testing.assert_array_equal(bound.result.to_host(), first.T)
     mx_matmul.submit(a, b, out=bound.result.device.empty(T.bf16, 4, 8)).wait()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("m,n,k,epilogue", [(4096, 2176, 512, "none"), (2176, 4224, 544, "bias"), (4100, 2100, 1056, "silu"),
+                                            (2304, 4112, 1024, "bias_relu")])
+def test_many_tiles_and_nothing_else_is_written(device, kind, m, n, k, epilogue):
+    """Products of the 256 x 256 tiles, whole and ragged, rows that end inside a slab; sizes that leave a quarter of the
+    last tiles past the end of the result. The memory behind the result stays."""
+    rng = np.random.default_rng(m + n)
+    a, b = random_mx(rng, m, k, 1), random_mx(rng, n, k, 1)
+    bias, exact = words(rng.uniform(-2, 2, n), kind)
+    host = np.full(m * n + 512 * n, 77, np.uint16 if kind == "bf16" else {"f32": np.float32, "f16": np.float16}[kind])
+    held = device.to_device(host, TYPES[kind])
+    out = HIPTensor(device, held.pointer, TYPES[kind], (m, n), owner=held)
+    mx_matmul(to_device(device, *a, k), to_device(device, *b, k), epilogue=epilogue, out=out,
+              bias=device.to_device(bias, TYPES[kind]) if "bias" in epilogue else None)
+    assert (held.to_host()[m * n:] == 77).all()
+    activation = epilogue.removeprefix("bias_")
+    rows = np.r_[0:3, 127:130, 255:258, m - 130:m]  # the first rows of blocks, and the last tile's
+    check(values(out)[rows], mx.decode(*a, k)[rows], mx.decode(*b, k), kind, exact if "bias" in epilogue else None,
+          activation if activation in ("silu", "relu") else None)
