@@ -759,15 +759,16 @@ int krn_mx_gemm(const void* a, const void* a_scales, const void* b, const void* 
                 void* workspace, int64_t workspace_bytes, void* stream) {
   MxCall g{};
   if (!mx_epilogue(g.e, out_kind, nops, ops, scalars, vectors)) return -1;
-  // 256 rows of codes are addressed by 31-bit offsets; tiles as a launch's threads allow
-  if (m < 0 || n < 0 || k < 1 || k >= (int64_t)1 << 23 || m >= (int64_t)1 << 31 || n >= (int64_t)1 << 31 ||
-      ((m + 127) / 128) * ((n + 127) / 128) >= (int64_t)1 << 24) {
-    krn_set_error("mx_gemm: %lld x %lld x %lld; rows of 1 to 2^23 - 1 values, m and n below 2^31, fewer than 2^24 tiles of "
-                  "128 x 128", (long long)m, (long long)n, (long long)k);
+  // 256 rows of codes are addressed by 31-bit offsets; a launch has fewer than 2^32 threads, and the most here are 512 for 32
+  // columns (few rows) and 256 for a tile of 64 x 64
+  if (m < 0 || n < 0 || k < 1 || k >= (int64_t)1 << 23 || m >= (int64_t)1 << 28 || n >= (int64_t)1 << 28 ||
+      ((m + 63) / 64) * ((n + 63) / 64) >= (int64_t)1 << 24) {
+    krn_set_error("mx_gemm: %lld x %lld x %lld; rows of 1 to 2^23 - 1 values, m and n below 2^28, fewer than 2^24 tiles of "
+                  "64 x 64", (long long)m, (long long)n, (long long)k);
     return -1;
   }
-  if ((uintptr_t)a % 16 != 0 || (uintptr_t)b % 16 != 0) {
-    krn_set_error("mx_gemm: codes start at a 16-byte aligned address");
+  if ((uintptr_t)a % 16 != 0 || (uintptr_t)b % 16 != 0 || (uintptr_t)workspace % 16 != 0) {
+    krn_set_error("mx_gemm: codes and workspace start at 16-byte aligned addresses");
     return -1;
   }
   if (m == 0 || n == 0) return 0;

@@ -176,3 +176,20 @@ def test_the_entry_points_refuse_before_any_device_call():
     assert "workspace" in layer(ws=None) and "workspace" in layer(nbytes=workspace(2, 3, 64, 48, 4, 2) - 1)
     assert "shares memory" in layer(y=x)
     assert workspace(2, 65, 64, 48, 4, 2) == 0 and workspace(2, 64, 64, 48, 4, 2) > 0
+
+
+@needs_library
+def test_the_product_refuses_launches_of_too_many_threads_and_a_workspace_at_odd_places():
+    """A launch holds fewer than 2^32 threads: 512 for 32 columns of a few rows, 256 for a tile of 64 x 64."""
+    library = ctypes.CDLL(str(LIBRARY))
+    library.krn_amd_last_error.restype = ctypes.c_char_p
+    p, i64 = ctypes.c_void_p, ctypes.c_int64
+
+    def refused(m, n, workspace=None):
+        assert library.krn_mx_gemm(p(1 << 30), p(1 << 32), p(1 << 40), p(1 << 45), p(1 << 46), 2, i64(m), i64(n), i64(32), 0, None,
+                                   None, None, workspace, i64(0), None) == -1
+        return library.krn_amd_last_error().decode()
+
+    assert "below 2^28" in refused(32, 1 << 28) and "below 2^28" in refused(1 << 28, 8)
+    assert "2^24 tiles" in refused(64 * 4096, 64 * 4096)
+    assert "aligned" in refused(70, 100, p((1 << 41) + 8))
