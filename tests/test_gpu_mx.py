@@ -9,6 +9,7 @@ import pytest
 from krn_amd import T
 from krn_amd.dtypes import BF16, F16, F32, U8
 from krn_amd.lib import MxMatrix, mx_dequantize, mx_matmul, mx_quantize
+from krn_amd.runtime import library
 from krn_amd.runtime.hip import HIPTensor
 from oracle import mx
 from oracle.numerics import bf16_values, bf16_words
@@ -158,6 +159,25 @@ def test_products(device, kind, m, n, k):
     got = mx_matmul(to_device(device, *a, k), to_device(device, *b, k), dtype=TYPES[kind])
     assert got.dtype == TYPES[kind] and got.shape == (m, n)
     check(values(got), mx.decode(*a, k), mx.decode(*b, k), kind)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("m,n,k,epilogue", [(70, 100, 8192, "none"), (128, 133, 14336, "bias_gelu"), (40, 260, 5000, "bias")])
+def test_products_whose_k_is_split(device, kind, m, n, k, epilogue):
+    """Few tiles and a long K: parts of K in planes of the workspace, added with the epilogue by a second kernel. Without
+    a workspace another kernel gives the product."""
+    assert library.mx_gemm_workspace(m, n, k) > 0
+    rng = np.random.default_rng(m)
+    a, b = random_mx(rng, m, k, 1), random_mx(rng, n, k, 1)
+    bias, exact = words(rng.uniform(-2, 2, n), kind)
+    left, right, vector = to_device(device, *a, k), to_device(device, *b, k), device.to_device(bias, TYPES[kind])
+    got = mx_matmul(left, right, epilogue=epilogue, dtype=TYPES[kind], bias=vector if "bias" in epilogue else None)
+    wide, activation = (mx.decode(*a, k), mx.decode(*b, k)), "gelu" if "gelu" in epilogue else None
+    check(values(got), *wide, kind, exact if "bias" in epilogue else None, activation)
+    out = device.empty(TYPES[kind], m, n)
+    library.mx_gemm_call(left.pointers, right.pointers, out.pointer, TYPES[kind], m, n, k, [], 0)(
+        0, device.default_stream.handle)
+    check(values(out), *wide, kind)
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
