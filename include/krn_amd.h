@@ -163,6 +163,10 @@ int krn_mx_gemm(const void* a, const void* a_scales, const void* b, const void* 
                 void* workspace, int64_t workspace_bytes, void* stream);
 int64_t krn_mx_gemm_workspace(int64_t m, int64_t n, int64_t k);
 
+/* The name of the kernel that such a call runs (few_16x16 to quad_256x256: the rows and columns of a workgroup), with an
+ * activation in its epilogue or without; empty where none runs. Nothing is launched. */
+const char* krn_mx_gemm_kernel(int64_t m, int64_t n, int64_t k, int activation, int64_t workspace_bytes);
+
 /* A mixture-of-experts layer for `tokens` <= 64 tokens: y_t = sum over the top_k experts e of token t of
  * w_te * down_e (silu(gate_e x_t) * up_e x_t). x is tokens x hidden and router experts x hidden, of kind KRN_F16 or KRN_BF16;
  * a token's experts are those of the top_k largest x_t . router_e (ties to the lower index, NaN the largest), w_t the

@@ -685,6 +685,8 @@ static bool mx_epilogue(Epilogue& e, int out_kind, int nops, const int* ops, con
 
 // Few rows: 16 x (16 NT) columns a workgroup; then tiles, by their stages; then the four-wave loop on 256 x 256 tiles
 enum MxShape : int { FEW_16x16, FEW_16x32, FEW_16x64, FEW_32x16, FEW_32x32, TILE_64_SHORT, TILE_64, TILE_64_DEEP, TILE_64x128, TILE_128, QUAD };
+static const char* const SHAPE_NAMES[] = {"few_16x16", "few_16x32", "few_16x64", "few_32x16", "few_32x32", "tile_64x64_short",
+                                          "tile_64x64", "tile_64x64_deep", "tile_64x128", "tile_128x128", "quad_256x256"};
 struct MxPlan {
   int shape, parts;
   int64_t workspace;
@@ -696,7 +698,8 @@ static MxPlan mx_plan(int64_t m, int64_t n, int64_t nb, bool activation, int64_t
   // 8192 8.7 / 8.3 / 12.4, 16 x 14336 x 4096 11.3 / 9.3 / 8.7, 8 x 28672 x 8192 35.8 / 32.2 / 31.5; 24 x 4096 x 4096 5.5 /
   // 6.9, 32 x 8192 x 8192 15.9 / 11.7, tiles of 64 x 64 7.7 and 11.9.
   if (m <= 16) return {n >= 64 * 224 ? FEW_16x64 : n >= 32 * 256 ? FEW_16x32 : FEW_16x16, 1, 0};
-  if (m <= 32) return {n >= 32 * 256 ? FEW_32x32 : FEW_32x16, 1, 0};
+  // A launch has fewer than 2^32 threads: 512 for 32 columns reach that at the last n below 2^28, which tiles take.
+  if (m <= 32 && n <= ((int64_t)1 << 28) - 32) return {n >= 32 * 256 ? FEW_32x32 : FEW_32x16, 1, 0};
   // Estimated microseconds beyond a launch: what a slab takes the CU that holds most workgroups, measured at K = 8192
   // (64 x 64 tiles, 256 workgroups 14.1 us, 512 21.8, 1024 39.1; eight stages 13.5, 24.5; 64 x 128 17.2, 35.3; 128 x 128 22.4,
   // 52.3; 256 x 256 tiles, 128 of them 52.6, 256 66.3), and what parts add: their planes' way to the second launch and back
@@ -752,6 +755,12 @@ static int launch_planned(const MxPlan& p, const MxCall& g) {
   return launched("mx_gemm");
 }
 
+// Whether a product of these sizes is taken
+static bool mx_sizes(int64_t m, int64_t n, int64_t k) {
+  return m >= 0 && n >= 0 && k >= 1 && k < (int64_t)1 << 23 && m < (int64_t)1 << 28 && n < (int64_t)1 << 28 &&
+         ((m + 63) / 64) * ((n + 63) / 64) < (int64_t)1 << 24;
+}
+
 extern "C" {
 
 int krn_mx_gemm(const void* a, const void* a_scales, const void* b, const void* b_scales, void* c, int out_kind, int64_t m,
@@ -759,10 +768,9 @@ int krn_mx_gemm(const void* a, const void* a_scales, const void* b, const void* 
                 void* workspace, int64_t workspace_bytes, void* stream) {
   MxCall g{};
   if (!mx_epilogue(g.e, out_kind, nops, ops, scalars, vectors)) return -1;
-  // 256 rows of codes are addressed by 31-bit offsets; a launch has fewer than 2^32 threads, and the most here are 512 for 32
-  // columns (few rows) and 256 for a tile of 64 x 64
-  if (m < 0 || n < 0 || k < 1 || k >= (int64_t)1 << 23 || m >= (int64_t)1 << 28 || n >= (int64_t)1 << 28 ||
-      ((m + 63) / 64) * ((n + 63) / 64) >= (int64_t)1 << 24) {
+  // 256 rows of codes are addressed by 31-bit offsets; a launch has fewer than 2^32 threads, 256 for a tile of 64 x 64 (few rows:
+  // mx_plan)
+  if (!mx_sizes(m, n, k)) {
     krn_set_error("mx_gemm: %lld x %lld x %lld; rows of 1 to 2^23 - 1 values, m and n below 2^28, fewer than 2^24 tiles of "
                   "64 x 64", (long long)m, (long long)n, (long long)k);
     return -1;
@@ -789,6 +797,11 @@ int64_t krn_mx_gemm_workspace(int64_t m, int64_t n, int64_t k) {
   if (m <= 0 || n <= 0 || k <= 0) return 0;
   const int64_t plain = mx_plan(m, n, mx_blocks(k), false, INT64_MAX).workspace, with = mx_plan(m, n, mx_blocks(k), true, INT64_MAX).workspace;
   return plain > with ? plain : with;
+}
+
+const char* krn_mx_gemm_kernel(int64_t m, int64_t n, int64_t k, int activation, int64_t workspace_bytes) {
+  if (!mx_sizes(m, n, k) || m == 0 || n == 0) return "";
+  return SHAPE_NAMES[mx_plan(m, n, mx_blocks(k), activation != 0, workspace_bytes).shape];
 }
 
 }  // extern "C"

@@ -87,6 +87,8 @@ def lib() -> ctypes.CDLL:
     ]  # fmt: skip
     handle.krn_mx_gemm_workspace.restype = c_int64
     handle.krn_mx_gemm_workspace.argtypes = [c_int64, c_int64, c_int64]
+    handle.krn_mx_gemm_kernel.restype = c_char_p
+    handle.krn_mx_gemm_kernel.argtypes = [c_int64, c_int64, c_int64, c_int, c_int64]
     handle.krn_moe.restype = c_int
     handle.krn_moe.argtypes = [
         c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
@@ -230,6 +232,12 @@ def mx_dequantize_call(codes: int, scales: int, dtype: Dtype, y: int, rows: int,
 def mx_gemm_workspace(m: int, n: int, k: int) -> int:
     """Bytes of device workspace `mx_gemm_call` of these sizes uses."""
     return lib().krn_mx_gemm_workspace(m, n, k)
+
+
+def mx_gemm_kernel(m: int, n: int, k: int, activation: bool = False, workspace_bytes: int | None = None) -> str:
+    """The kernel that `mx_gemm_call` of these sizes runs, by default with all the workspace it uses."""
+    held = mx_gemm_workspace(m, n, k) if workspace_bytes is None else workspace_bytes
+    return lib().krn_mx_gemm_kernel(m, n, k, activation, held).decode()
 
 
 def mx_gemm_call(a: tuple[int, int], b: tuple[int, int], c: int, out_dtype: Dtype, m: int, n: int, k: int,

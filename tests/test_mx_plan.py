@@ -1,0 +1,29 @@
+"""Which kernel an MX product runs, and how large its launch is: host arithmetic, no GPU."""
+
+import pytest
+
+from krn_amd.runtime import library
+from tests.test_library import LIBRARY
+
+pytestmark = pytest.mark.skipif(not LIBRARY.exists(), reason="libkrn_amd.so is not built")
+
+# rows and columns of a workgroup (rows 0: all of them), its threads
+KERNELS = {"few_16x16": (0, 16, 512), "few_16x32": (0, 32, 512), "few_16x64": (0, 64, 256), "few_32x16": (0, 16, 256),
+           "few_32x32": (0, 32, 512), "tile_64x64_short": (64, 64, 256), "tile_64x64": (64, 64, 256),
+           "tile_64x64_deep": (64, 64, 256), "tile_64x128": (64, 128, 256), "tile_128x128": (128, 128, 256),
+           "quad_256x256": (256, 256, 256)}
+LAST = (1 << 28) - 1
+
+
+@pytest.mark.parametrize("activation", [False, True])
+@pytest.mark.parametrize("k", [1, 32, 512, 8192])
+@pytest.mark.parametrize("m,n", [(1, LAST), (16, LAST), (17, LAST), (32, LAST), (32, LAST - 30), (32, LAST - 31), (33, 1 << 27),
+                                 (1 << 27, 33), (LAST, 1), (LAST, 32), (LAST, 64), (64 * 4095, 64 * 4095)])
+def test_a_launch_holds_fewer_than_2_to_the_32_threads(m, n, k, activation):
+    rows, cols, threads = KERNELS[library.mx_gemm_kernel(m, n, k, activation, 0)]
+    assert (-(-m // rows) if rows else 1) * -(-n // cols) * threads < 1 << 32
+
+
+def test_no_kernel_runs_for_sizes_that_are_refused_or_empty():
+    for m, n, k in [(0, 5, 32), (5, 0, 32), (-1, 5, 32), (5, 5, 0), (5, 5, 1 << 23), (1 << 28, 5, 32), (5, 1 << 28, 32)]:
+        assert library.mx_gemm_kernel(m, n, k) == ""
