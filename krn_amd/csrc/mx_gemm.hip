@@ -694,10 +694,19 @@ struct MxPlan {
 
 static MxPlan mx_plan(int64_t m, int64_t n, int64_t nb, bool activation, int64_t workspace) {
   const int64_t slabs = (nb + SLAB - 1) / SLAB;
-  // Up to 32 rows: wider workgroups read A less often, narrower ones fill the chip (us, on 16 / 32 / 64 columns): 1 x 8192 x
-  // 8192 8.7 / 8.3 / 12.4, 16 x 14336 x 4096 11.3 / 9.3 / 8.7, 8 x 28672 x 8192 35.8 / 32.2 / 31.5; 24 x 4096 x 4096 5.5 /
-  // 6.9, 32 x 8192 x 8192 15.9 / 11.7, tiles of 64 x 64 7.7 and 11.9.
-  if (m <= 16) return {n >= 64 * 224 ? FEW_16x64 : n >= 32 * 256 ? FEW_16x32 : FEW_16x16, 1, 0};
+  // Up to 32 rows: wider workgroups read A less often, narrower ones fill the chip. Up to 16 rows (us, on 16 / 32 / 64 columns,
+  // three sets of operands in turn): 1 x 8192 x 8192 9.1 / 8.4 / 14.7, 1 x 14336 x 4096 8.5 / 8.0 / 9.2, 16 x 8192 x 4096 7.2 /
+  // 6.4 / 9.3, 16 x 14336 x 4096 11.4 / 9.5 / 9.8; one row at 9216 to 12288 columns is 10 % faster on 16, sixteen rows are equal.
+  // 64 columns pay from nine rows, where the launch fills its rounds: a CU holds three such workgroups, and takes twice as
+  // many of 32 columns (16 rows, K = 4096, on 32 / 64: n = 20480 12.8 / 14.3, 28672 16.1 / 14.7, 32768 16.2 / 15.4, 40960 21.5 /
+  // 22.3, 49152 28.0 / 26.1, 65536 38.5 / 44.1, 81920 47.1 / 49.0, 98304 55.7 / 52.1, 131072 72.9 / 73.4; 8 rows: 28672 14.5 / 14.2,
+  // with K = 8192 33.0 / 33.1; 1 row: 13.0 / 13.8).
+  if (m <= 16) {
+    const int64_t wide = (n + 64 * 256 - 1) / (64 * 256), half = (n + 32 * 256 - 1) / (32 * 256);  // workgroups a CU
+    if (m > 8 && (wide == 2 || wide % 3 == 0) && 2 * wide <= half) return {FEW_16x64, 1, 0};
+    return {n >= 32 * 256 ? FEW_16x32 : FEW_16x16, 1, 0};
+  }
+  // (us, on 16 / 32 columns: 24 x 4096 x 4096 5.5 / 6.9, 32 x 8192 x 8192 15.9 / 11.7, tiles of 64 x 64 7.7 and 11.9)
   // A launch has fewer than 2^32 threads: 512 for 32 columns reach that at the last n below 2^28, which tiles take.
   if (m <= 32 && n <= ((int64_t)1 << 28) - 32) return {n >= 32 * 256 ? FEW_32x32 : FEW_32x16, 1, 0};
   // Estimated microseconds beyond a launch: what a slab takes the CU that holds most workgroups, measured at K = 8192

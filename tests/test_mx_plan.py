@@ -27,3 +27,13 @@ def test_a_launch_holds_fewer_than_2_to_the_32_threads(m, n, k, activation):
 def test_no_kernel_runs_for_sizes_that_are_refused_or_empty():
     for m, n, k in [(0, 5, 32), (5, 0, 32), (-1, 5, 32), (5, 5, 0), (5, 5, 1 << 23), (1 << 28, 5, 32), (5, 1 << 28, 32)]:
         assert library.mx_gemm_kernel(m, n, k) == ""
+
+
+def test_the_columns_of_a_few_rows():
+    """One row to eight: 32 columns from 8192 on. Nine to sixteen: 64 where a CU gets two or a multiple of three of them."""
+    cols = {16: "few_16x16", 32: "few_16x32", 64: "few_16x64"}
+    for n in (1, 4096, 8191, 8192, 11008, 14336, 16384, 28672, 32768, 65536):
+        assert library.mx_gemm_kernel(1, n, 4096) == library.mx_gemm_kernel(8, n, 1000) == cols[16 if n < 8192 else 32]
+    for n, want in [(4096, 16), (8192, 32), (14336, 32), (16385, 32), (24576, 32), (24577, 64), (28672, 64), (32768, 64), (32769, 32),
+                    (40960, 32), (49152, 64), (65536, 32), (81920, 32), (98304, 64), (131072, 32)]:
+        assert library.mx_gemm_kernel(9, n, 4096) == library.mx_gemm_kernel(16, n, 777) == cols[want]
