@@ -694,6 +694,8 @@ struct MxPlan {
 
 static MxPlan mx_plan(int64_t m, int64_t n, int64_t nb, bool activation, int64_t workspace) {
   const int64_t slabs = (nb + SLAB - 1) / SLAB;
+  // A launch has fewer than 2^32 threads: 512 for 32 columns reach that at the last n below 2^28, which others take
+  constexpr int64_t MOST_32 = ((int64_t)1 << 28) - 32;
   // Up to 32 rows: wider workgroups read A less often, narrower ones fill the chip. Up to 16 rows (us, on 16 / 32 / 64 columns,
   // three sets of operands in turn): 1 x 8192 x 8192 9.1 / 8.4 / 14.7, 1 x 14336 x 4096 8.5 / 8.0 / 9.2, 16 x 8192 x 4096 7.2 /
   // 6.4 / 9.3, 16 x 14336 x 4096 11.4 / 9.5 / 9.8; one row at 9216 to 12288 columns is 10 % faster on 16, sixteen rows are equal.
@@ -703,12 +705,11 @@ static MxPlan mx_plan(int64_t m, int64_t n, int64_t nb, bool activation, int64_t
   // with K = 8192 33.0 / 33.1; 1 row: 13.0 / 13.8).
   if (m <= 16) {
     const int64_t wide = (n + 64 * 256 - 1) / (64 * 256), half = (n + 32 * 256 - 1) / (32 * 256);  // workgroups a CU
-    if (m > 8 && (wide == 2 || wide % 3 == 0) && 2 * wide <= half) return {FEW_16x64, 1, 0};
+    if (n > MOST_32 || (m > 8 && (wide == 2 || wide % 3 == 0) && 2 * wide <= half)) return {FEW_16x64, 1, 0};
     return {n >= 32 * 256 ? FEW_16x32 : FEW_16x16, 1, 0};
   }
   // (us, on 16 / 32 columns: 24 x 4096 x 4096 5.5 / 6.9, 32 x 8192 x 8192 15.9 / 11.7, tiles of 64 x 64 7.7 and 11.9)
-  // A launch has fewer than 2^32 threads: 512 for 32 columns reach that at the last n below 2^28, which tiles take.
-  if (m <= 32 && n <= ((int64_t)1 << 28) - 32) return {n >= 32 * 256 ? FEW_32x32 : FEW_32x16, 1, 0};
+  if (m <= 32 && n <= MOST_32) return {n >= 32 * 256 ? FEW_32x32 : FEW_32x16, 1, 0};
   // Estimated microseconds beyond a launch: what a slab takes the CU that holds most workgroups, measured at K = 8192
   // (64 x 64 tiles, 256 workgroups 14.1 us, 512 21.8, 1024 39.1; eight stages 13.5, 24.5; 64 x 128 17.2, 35.3; 128 x 128 22.4,
   // 52.3; 256 x 256 tiles, 128 of them 52.6, 256 66.3), and what parts add: their planes' way to the second launch and back
