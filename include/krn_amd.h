@@ -164,7 +164,8 @@ int krn_mx_gemm(const void* a, const void* a_scales, const void* b, const void* 
 int64_t krn_mx_gemm_workspace(int64_t m, int64_t n, int64_t k);
 
 /* The name of the kernel that such a call runs (few_16x16 to quad_256x256: the rows and columns of a workgroup), with an
- * activation in its epilogue or without; empty where none runs. Nothing is launched. */
+ * activation in its epilogue or without, followed by " in P parts" where K is split; empty where none runs. Nothing is
+ * launched; the text holds until the thread's next such call. */
 const char* krn_mx_gemm_kernel(int64_t m, int64_t n, int64_t k, int activation, int64_t workspace_bytes);
 
 /* A mixture-of-experts layer for `tokens` <= 64 tokens: y_t = sum over the top_k experts e of token t of

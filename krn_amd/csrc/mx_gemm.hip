@@ -811,7 +811,11 @@ int64_t krn_mx_gemm_workspace(int64_t m, int64_t n, int64_t k) {
 
 const char* krn_mx_gemm_kernel(int64_t m, int64_t n, int64_t k, int activation, int64_t workspace_bytes) {
   if (!mx_sizes(m, n, k) || m == 0 || n == 0) return "";
-  return SHAPE_NAMES[mx_plan(m, n, mx_blocks(k), activation != 0, workspace_bytes).shape];
+  const MxPlan p = mx_plan(m, n, mx_blocks(k), activation != 0, workspace_bytes);
+  if (p.parts == 1) return SHAPE_NAMES[p.shape];
+  thread_local char name[48];
+  snprintf(name, sizeof name, "%s in %d parts", SHAPE_NAMES[p.shape], p.parts);
+  return name;
 }
 
 }  // extern "C"
