@@ -44,8 +44,9 @@ inline bool share_memory(const void* a, int64_t a_bytes, const void* b, int64_t 
 }
 
 // A buffer resource over `bytes` bytes from `base` (raw 32-bit offsets, no stride, no swizzle; at most 2^31 - 1).
-// Loads past the end return zeros instead of touching memory: that is how the whole-tile GEMMs read the ragged
-// last rows of an operand.
+// Loads past the end return zeros instead of touching memory, and stores do nothing: that is how the whole-tile GEMMs read
+// the ragged last rows of an operand. The hardware holds the sum of lane and scalar offset against the end, without
+// wrapping (measured on gfx950 inside one allocation: scalar offsets of one, two and four times the end).
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t panel_rsrc(const void* base, int64_t bytes = 0x7fffffff) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)min(bytes, (int64_t)0x7fffffff),
                                            0x00020000);

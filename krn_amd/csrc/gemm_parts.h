@@ -574,7 +574,7 @@ __device__ __forceinline__ void store16t_direct(const V4 (&acc)[8][8], Ops ops, 
   const uint32_t base_lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)base);
   const uint32_t base_hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(base >> 32));
   const void* region = (const void*)(((uint64_t)base_hi << 32) | (uint64_t)base_lo);
-  const __amdgpu_buffer_rsrc_t out = panel_rsrc(region, rows * ldc * 2);  // stores to rows past `rows` do nothing
+  const __amdgpu_buffer_rsrc_t out = panel_rsrc(region, rows * ldc * 2);  // rows past `rows`, whole blocks too, store nothing
   // after the exchange below, lane group g holds the 16 columns of block 4 jj + g of its row: two 16-byte pieces
   const uint32_t lane_off = (uint32_t)((r16 * ldc + 16 * g) * 2);
 #pragma unroll
