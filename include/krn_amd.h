@@ -155,7 +155,7 @@ int krn_mx_dequantize(const void* codes, const void* scales, int kind, void* y, 
 
 /* C[m, n] = epilogue(sum_k A[m, k] * B[n, k]) of two MX matrices, float32 sums; out_kind KRN_F32, KRN_F16 or KRN_BF16, the
  * epilogue as for krn_gemm_nt. k is below 2^23, m and n below 2^28, tiles of 64 x 64 fewer than 2^24. C shares no memory
- * with an operand. A workspace of krn_mx_gemm_workspace bytes (16-byte aligned, no preparation, not touched by other work
+ * with an operand or a vector. A workspace of krn_mx_gemm_workspace bytes (16-byte aligned, no preparation, not touched by other work
  * until this call's has run; calls on one stream may share one) lets K be split over workgroups; with less, or none,
  * another kernel runs. */
 int krn_mx_gemm(const void* a, const void* a_scales, const void* b, const void* b_scales, void* c, int out_kind, int64_t m,

@@ -796,6 +796,13 @@ int krn_mx_gemm(const void* a, const void* a_scales, const void* b, const void* 
     krn_set_error("mx_gemm: the result shares memory with an operand");
     return -1;
   }
+  for (int i = 0; i < nops; ++i) {
+    const int op = ops[i] & ((1 << VEC_KIND_SHIFT) - 1), size = ops[i] >> VEC_KIND_SHIFT ? 2 : 4;
+    if (op < RELU && op % 3 != 0 && share_memory(c, c_bytes, vectors[i], (op % 3 == 1 ? m : n) * size)) {
+      krn_set_error("mx_gemm: the result shares memory with a vector of the epilogue");
+      return -1;
+    }
+  }
   g.a = (const uint8_t*)a, g.as = (const uint8_t*)a_scales, g.b = (const uint8_t*)b, g.bs = (const uint8_t*)b_scales;
   g.c = c, g.m = m, g.n = n, g.nb = (int)nb, g.workspace = workspace, g.stream = (hipStream_t)stream;
   bool activation = false;

@@ -85,7 +85,7 @@ def mx_dequantize(a, *, dtype: Dtype = BF16, out=None) -> Work:
 def mx_matmul(a, b, *, epilogue: Epilogue = Epilogue.NONE, bias=None, dtype: Dtype = BF16, out=None) -> Work:
     """`a @ b.T` of the MX matrices a (m, k) and b (n, k), the layout of a linear layer's weight, with an epilogue of
     `lib.matmul`; float32 sums, rounded once to f32, f16 or bf16 (`dtype`, or the type of `out`). A bias is a vector of
-    n values of the result's type. `out` shares no memory with an operand."""
+    n values of the result's type. `out` shares no memory with an operand or the bias."""
     epilogue = Epilogue(epilogue)
     (m, k), (n, kb) = matrix(a, "a").shape, matrix(b, "b").shape
     if k != kb:
