@@ -105,8 +105,10 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// The experts of token t, by one wave: lane j < top_k gets choice j and its weight. EPL: experts a lane
-template <int EPL>
+// The experts of token t, by one wave: lane j < top_k gets choice j and its weight. EPL: experts a lane. WAVES16: one of sixteen
+// waves, whose 128 registers do not hold all loads of sixteen experts (67 spilled: 64 tokens, 8 of 1024 experts 170 -> 84 us
+// for the layer); one of eight has room for them (2 tokens, 16 of 1024 29.1, 32 loads at a time 29.8)
+template <int EPL, bool WAVES16>
 __device__ __forceinline__ void choose(const float* __restrict__ partial, int t, int T, int E, int top_k, int lane, int& pick,
                                        float& weight) {
   uint32_t key[EPL];  // expert lane + 64 i, 0 once chosen and past the last
@@ -120,7 +122,8 @@ __device__ __forceinline__ void choose(const float* __restrict__ partial, int t,
 #pragma unroll
     for (int p = 1; p < PARTS; ++p) sum += v[p];
     key[i] = e < E ? ordered(sum) : 0;
-    if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // 32 loads at a time: all of them do not fit the registers
+    if (WAVES16 && EPL > 4 && i % 4 == 3)  // 32 loads at a time, the address of the next after their sums
+      asm volatile("" : "+s"(partial) : "v"(key[i]), "v"(key[i - 1]), "v"(key[i - 2]), "v"(key[i - 3]));
   }
   float mine = -INFINITY;  // lane j: the logit of choice j
   pick = 0;
@@ -157,7 +160,7 @@ __global__ __launch_bounds__(1024) void moe_route(const float* __restrict__ part
   for (int t = wave; t < T; t += 16) {
     int pick;
     float w;
-    choose<EPL>(partial, t, T, E, top_k, lane, pick, w);
+    choose<EPL, true>(partial, t, T, E, top_k, lane, pick, w);
     if (lane < top_k) {
       chosen[t * top_k + lane] = pick, weight[t * top_k + lane] = w;
       atomicOr(&mask[pick], 1ull << t);
@@ -206,7 +209,7 @@ __device__ __forceinline__ void route_few(FewRouting& out, const float* __restri
   if (wave < T) {
     int pick;
     float w;
-    choose<EPL>(partial, wave, T, E, top_k, lane, pick, w);
+    choose<EPL, false>(partial, wave, T, E, top_k, lane, pick, w);
     if (lane < top_k) out.chosen[wave * top_k + lane] = pick, out.given[wave * top_k + lane] = w;
   }
   __syncthreads();
