@@ -156,8 +156,9 @@ __device__ __forceinline__ void spread_scales(const u32x4& d, uint32_t (&out)[4]
 #pragma unroll
   for (int n = 0; n < 6; ++n) s.step(n, d, out);
 }
+
 // An activation of four values. Out of line, so that its registers are not the store's as well: three workgroups of 64 x 64
-// tiles share a CU instead of two (1000 x 3001 x 777 with bias and gelu 22.7 -> 18.9 us; silu above 257 -> 297)
+// tiles share a CU instead of two (1000 x 3001 x 777 with bias and gelu 22.7 -> 18.9 us)
 __device__ __noinline__ f32x4 activate4(f32x4 x, int op) {
 #define KRN_ALL(OP) f32x4{activation(OP, x[0]), activation(OP, x[1]), activation(OP, x[2]), activation(OP, x[3])}
   if (op == RELU) return KRN_ALL(RELU);
@@ -167,7 +168,9 @@ __device__ __noinline__ f32x4 activate4(f32x4 x, int op) {
 
 // One 32 x 32 block from its patch through the epilogue to C, rows at any alignment: lane l has columns 16 (l & 1) .. + 15 of
 // row l / 2. Out of line, each wave storing several blocks. What an operation does is decided once for four or more
-// values (4096 x 14336 x 4096 with silu: 566 us decided value by value, 297 here).
+// values. WIDE: the four-wave loop's, which has a CU to itself: activations of sixteen values in line, whose chains overlap
+// (4096 x 14336 x 4096 with silu: 297 us in calls of four, 253; bias and gelu 515, 450).
+template <bool WIDE>
 __device__ __noinline__ void store_patch(uint32_t* patch, void* C, int64_t ldc, int64_t row0, int64_t col0, int64_t M,
                                          int64_t N, const Epilogue& e, int lane) {
   __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the patch is written before any lane reads it
@@ -187,7 +190,11 @@ __device__ __noinline__ void store_patch(uint32_t* patch, void* C, int64_t ldc, 
   for (int i = 0; i < e.nops; ++i) {
     const int op = e.op[i] & ((1 << VEC_KIND_SHIFT) - 1), kind = e.op[i] >> VEC_KIND_SHIFT;
 #define KRN_ALL(x) _Pragma("unroll") for (int c = 0; c < 16; ++c) v[c] = x
-    if (op >= RELU) {
+    if (WIDE && op >= RELU) {
+      if (op == RELU) { KRN_ALL(activation(RELU, v[c])); }
+      else if (op == GELU) { KRN_ALL(activation(GELU, v[c])); }
+      else { KRN_ALL(activation(SILU, v[c])); }
+    } else if (op >= RELU) {
 #pragma unroll
       for (int c = 0; c < 16; c += 4) {
         const f32x4 x = activate4(f32x4{v[c], v[c + 1], v[c + 2], v[c + 3]}, op);
@@ -404,7 +411,7 @@ __global__ __launch_bounds__(256) void mx_tile(const uint8_t* __restrict__ A, co
 #pragma unroll
         for (int q = 0; q < 2; ++q)
           *reinterpret_cast<f32x4*>(patch + (16 * p + r) * PATCH_STRIDE + 16 * q + 4 * g) = acc[i + p][k + q];
-      store_patch(patch, C, ldc, m0 + wm * (16 * TM) + 16 * i, n0 + wn * (16 * TN) + 16 * k, M, N, local, lane);
+      store_patch<false>(patch, C, ldc, m0 + wm * (16 * TM) + 16 * i, n0 + wn * (16 * TN) + 16 * k, M, N, local, lane);
     }
 }
 
@@ -638,7 +645,7 @@ __global__ __launch_bounds__(256, 1) void mx_quad(const uint8_t* __restrict__ A,
 #pragma unroll
         for (int q = 0; q < 2; ++q)
           *reinterpret_cast<f32x4*>(patch + (16 * p + r16) * PATCH_STRIDE + 16 * q + 4 * g4) = agpr_block(acc[i + p][k + q]);
-      store_patch(patch, C, ldc, row0 + 16 * i, col0 + 16 * k, M, N, local, lane);
+      store_patch<true>(patch, C, ldc, row0 + 16 * i, col0 + 16 * k, M, N, local, lane);
     }
 }
 
