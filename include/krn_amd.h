@@ -155,9 +155,9 @@ int krn_mx_dequantize(const void* codes, const void* scales, int kind, void* y, 
 
 /* C[m, n] = epilogue(sum_k A[m, k] * B[n, k]) of two MX matrices, float32 sums; out_kind KRN_F32, KRN_F16 or KRN_BF16, the
  * epilogue as for krn_gemm_nt. k is below 2^23, m and n below 2^28, tiles of 64 x 64 fewer than 2^24. C shares no memory
- * with an operand or a vector. A workspace of krn_mx_gemm_workspace bytes (16-byte aligned, no preparation, not touched by other work
- * until this call's has run; calls on one stream may share one) lets K be split over workgroups; with less, or none,
- * another kernel runs. */
+ * with an operand or a vector. A workspace of krn_mx_gemm_workspace bytes (16-byte aligned, no preparation, not touched by
+ * other work until this call's has run; calls on one stream may share one) lets K be split over workgroups; with less, or
+ * none, another kernel runs. */
 int krn_mx_gemm(const void* a, const void* a_scales, const void* b, const void* b_scales, void* c, int out_kind, int64_t m,
                 int64_t n, int64_t k, int nops, const int* ops, const float* scalars, const void* const* vectors,
                 void* workspace, int64_t workspace_bytes, void* stream);
@@ -173,8 +173,9 @@ const char* krn_mx_gemm_kernel(int64_t m, int64_t n, int64_t k, int activation, 
  * a token's experts are those of the top_k largest x_t . router_e (ties to the lower index, NaN the largest), w_t the
  * softmax of these logits. gate_up is the MX matrix of experts * 2 * inner rows of `hidden` values (an expert's gate rows,
  * then its up rows), down that of experts * hidden rows of `inner` values. y is of x's kind and shares no memory with the
- * inputs. At most 1024 experts, top_k <= 16. The workspace holds krn_moe_workspace bytes, needs no preparation, is 16-byte
- * aligned and not touched by other work until this call's has run; calls on one stream may share one. */
+ * inputs. Logits are float32 sums, inner values are rounded to 2^-16. At most 1024 experts, top_k <= 16. The workspace
+ * holds krn_moe_workspace bytes, needs no preparation, is 16-byte aligned and not touched by other work until this call's
+ * has run; calls on one stream may share one. */
 int krn_moe(int kind, const void* x, const void* router, const void* gate_up, const void* gate_up_scales, const void* down,
             const void* down_scales, void* y, int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int64_t top_k,
             void* workspace, int64_t workspace_bytes, void* stream);

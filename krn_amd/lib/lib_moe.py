@@ -15,7 +15,9 @@ def moe(x, router, gate_up, down, *, top_k: int, out=None) -> Work:
     experts are those with the largest x_t . router_e, ties going to the lower index and NaN counting as the largest; w_t is
     the softmax of those logits. `gate_up` is the MxMatrix of experts * 2 * inner rows of hidden values, for every expert
     its inner gate rows and then its inner up rows; `down` the one of experts * hidden rows of inner values. At most 1024
-    experts and 16 of them for a token. The result, (tokens, hidden) of x's type, shares no memory with the inputs."""
+    experts and 16 of them for a token. Logits are float32 sums, so experts whose logits differ by less than such a sum's
+    error may change places; the inner values are rounded to 2^-16, everything else is float32 up to the result, (tokens,
+    hidden) of x's type, which shares no memory with the inputs."""
     tensor(x, "x", 2, (F16, BF16))
     tensor(router, "router", 2, (x.dtype,))
     (tokens, hidden), experts, inner = x.shape, router.shape[0], matrix(down, "down").shape[1]
