@@ -181,6 +181,39 @@ int krn_moe(int kind, const void* x, const void* router, const void* gate_up, co
             void* workspace, int64_t workspace_bytes, void* stream);
 int64_t krn_moe_workspace(int kind, int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int64_t top_k);
 
+/* A paged key-value cache: `keys` and `values` are each pages x kv_heads x page x d, of kind KRN_F16 or KRN_BF16, d 64 or 128,
+ * page a power of two from 16 to 65536, 16-byte aligned. The sequences of a step: `lengths` (sequences) counts the keys of each,
+ * those of its newest tokens included, and `table` (sequences x width) numbers the pages that it owns: key j of sequence i lies
+ * in row j % page of page table[i, j / page]. The step's tokens are packed; those of sequence i are starts[i] to
+ * starts[i + 1] - 1 (`starts` has sequences + 1 entries and does not decrease) or, with starts NULL, `step` for every sequence
+ * (tokens = step * sequences). Its last token has position lengths[i] - 1. All three arrays are int32 on the device and are read
+ * when the kernels run. They are checked there: a token that no range holds belongs to no sequence and what would be written
+ * for it stays as it was, keys beyond width pages are not there, a page number outside of the cache reads as zeros and is
+ * not written. No counterpart in the reference, whose attention reads dense tensors.
+ *
+ * krn_rotary_append: qkv is tokens x (heads + 2 kv_heads) x d: query heads, key heads, value heads. Pair j of a query or key
+ * head, columns (j, j + rotary / 2) or (2j, 2j + 1) if interleaved, becomes magnitude (a cos t - b sin t, b cos t + a sin t)
+ * with t the token's position times frequency j, given as turns[j] = frequency / 2 pi mod 1 in 2^-64 (rotary / 2 of them);
+ * columns from `rotary` (even) on are copied. Queries go to q, tokens x heads x d, keys and values to their places in the
+ * cache. A token of a negative position, or one beyond its sequence's pages, is not stored. No two tokens share a place, and
+ * results share no memory with other tensors. */
+int krn_rotary_append(int kind, const void* qkv, void* q, void* keys, void* values, int64_t tokens, int64_t heads,
+                      int64_t kv_heads, int64_t d, int64_t pages, int64_t page, const int* starts, int64_t step,
+                      const int* lengths, const int* table, int64_t sequences, int64_t width, const uint64_t* turns,
+                      int64_t rotary, int interleaved, float magnitude, void* stream);
+
+/* o = softmax(scale q K^T) V, causal: a token at position p attends to its sequence's keys up to p, to the last `window` of them
+ * if that is not 0. q and o are tokens x heads x d; heads / kv_heads query heads share a key head; scale > 0. A token without
+ * keys gets zeros. o may be q itself and shares no other memory. A workspace of krn_cache_attention_workspace bytes (`packed`:
+ * with starts; 16-byte aligned, no preparation, not touched by other work until this call's has run; calls on one stream may
+ * share one) lets the keys of one token be split over workgroups; with less, or none, they stay in one. */
+int krn_cache_attention(int kind, const void* q, const void* keys, const void* values, void* o, int64_t tokens, int64_t heads,
+                        int64_t kv_heads, int64_t d, int64_t pages, int64_t page, const int* starts, int64_t step,
+                        const int* lengths, const int* table, int64_t sequences, int64_t width, float scale, int64_t window,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+int64_t krn_cache_attention_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t d, int64_t page, int packed,
+                                      int64_t sequences, int64_t width);
+
 /* The message of the calling thread's last failed call. */
 const char* krn_amd_last_error(void);
 

@@ -96,6 +96,18 @@ def lib() -> ctypes.CDLL:
     ]  # fmt: skip
     handle.krn_moe_workspace.restype = c_int64
     handle.krn_moe_workspace.argtypes = [c_int, c_int64, c_int64, c_int64, c_int64, c_int64]
+    handle.krn_rotary_append.restype = c_int
+    handle.krn_rotary_append.argtypes = [
+        c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64,
+        c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int, c_float, c_void_p,
+    ]  # fmt: skip
+    handle.krn_cache_attention.restype = c_int
+    handle.krn_cache_attention.argtypes = [
+        c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64,
+        c_void_p, c_void_p, c_int64, c_int64, c_float, c_int64, c_void_p, c_int64, c_void_p,
+    ]  # fmt: skip
+    handle.krn_cache_attention_workspace.restype = c_int64
+    handle.krn_cache_attention_workspace.argtypes = [c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int64, c_int64]
     return handle
 
 
@@ -272,5 +284,43 @@ def moe_call(dtype: Dtype, x: int, router: int, gate_up: tuple[int, int], down: 
 
     def call(workspace: int, stream: int) -> None:
         check(entry(*head, workspace, size, stream), "krn_moe")
+
+    return call
+
+
+def rotary_append_call(dtype: Dtype, qkv: int, q: int, keys: int, values: int, tokens: int, heads: int, kv_heads: int, d: int,
+                       pages: int, page: int, starts: int, step: int, lengths: int, table: int, sequences: int, width: int,
+                       turns: int, rotary: int, interleaved: bool, magnitude: float):
+    """The rotated append as a function of the stream, with the other arguments marshalled once."""
+    entry = lib().krn_rotary_append
+    head = (c_int(kind(dtype)), c_void_p(qkv), c_void_p(q), c_void_p(keys), c_void_p(values), c_int64(tokens), c_int64(heads),
+            c_int64(kv_heads), c_int64(d), c_int64(pages), c_int64(page), c_void_p(starts), c_int64(step), c_void_p(lengths),
+            c_void_p(table), c_int64(sequences), c_int64(width), c_void_p(turns), c_int64(rotary), c_int(interleaved),
+            c_float(magnitude))
+
+    def call(stream: int) -> None:
+        check(entry(*head, stream), "krn_rotary_append")
+
+    return call
+
+
+def cache_attention_workspace(tokens: int, heads: int, kv_heads: int, d: int, pages: int, page: int, starts: int, step: int,
+                              lengths: int, table: int, sequences: int, width: int) -> int:
+    """Bytes of device workspace `cache_attention_call` of these sizes uses."""
+    return lib().krn_cache_attention_workspace(tokens, heads, kv_heads, d, page, int(starts != 0), sequences, width)
+
+
+def cache_attention_call(dtype: Dtype, q: int, keys: int, values: int, o: int, tokens: int, heads: int, kv_heads: int, d: int,
+                         pages: int, page: int, starts: int, step: int, lengths: int, table: int, sequences: int, width: int,
+                         scale: float, window: int, workspace_bytes: int):
+    """The attention over a cache as a function of the workspace and the stream, with the other arguments marshalled once."""
+    entry = lib().krn_cache_attention
+    head = (c_int(kind(dtype)), c_void_p(q), c_void_p(keys), c_void_p(values), c_void_p(o), c_int64(tokens), c_int64(heads),
+            c_int64(kv_heads), c_int64(d), c_int64(pages), c_int64(page), c_void_p(starts), c_int64(step), c_void_p(lengths),
+            c_void_p(table), c_int64(sequences), c_int64(width), c_float(scale), c_int64(window))
+    size = c_int64(workspace_bytes)
+
+    def call(workspace: int, stream: int) -> None:
+        check(entry(*head, workspace, size, stream), "krn_cache_attention")
 
     return call
