@@ -75,9 +75,27 @@ __global__ __launch_bounds__(64) void cache_attention_simple(CacheAttention c) {
 
 using namespace krn;
 
+static int launched() {
+  const hipError_t err = hipGetLastError();
+  if (err == hipSuccess) return 0;
+  krn_set_error("cache_attention launch: %s", hipGetErrorString(err));
+  return (int)err;
+}
+
+// The plan of a call without starts; without memory for its parts the keys of a sequence stay in one workgroup
+static TokenPlan plan_of(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t d, int64_t page, int64_t sequences,
+                         int64_t width, int64_t bytes) {
+  const int64_t step = tokens / sequences;
+  TokenPlan p = token_plan(step, heads / kv_heads, kv_heads, d, page, sequences, width);
+  if (p.bytes > bytes) p = token_plan(step, heads / kv_heads, kv_heads, d, page, sequences, 0);
+  return p;
+}
+
 extern "C" int64_t krn_cache_attention_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t d, int64_t page,
                                                  int packed, int64_t sequences, int64_t width) {
-  return 0;
+  if (packed || tokens <= 0 || sequences <= 0 || heads <= 0 || kv_heads <= 0 || width <= 0) return 0;
+  if (tokens / sequences * (heads / kv_heads) > TOKEN_ROWS) return 0;
+  return plan_of(tokens, heads, kv_heads, d, page, sequences, width, INT64_MAX).bytes;
 }
 
 extern "C" int krn_cache_attention(int kind, const void* q, const void* keys, const void* values, void* o, int64_t tokens,
@@ -116,6 +134,22 @@ extern "C" int krn_cache_attention(int kind, const void* q, const void* keys, co
   c.q = (const uint16_t*)q, c.o = (uint16_t*)o, c.heads = (int)heads;
   c.window = window > 0x7fffffff ? 0 : (int)window;
   c.scale = scale * 1.4426950408889634f;
+  if (!starts && step * (heads / kv_heads) <= TOKEN_ROWS) {
+    if ((uintptr_t)workspace % 16) {
+      krn_set_error("cache_attention: the workspace must be 16-byte aligned");
+      return -1;
+    }
+    const TokenPlan p = plan_of(tokens, heads, kv_heads, d, page, sequences, width, workspace ? workspace_bytes : 0);
+    if (p.workgroups * p.columns >= (int64_t)1 << 24) {
+      krn_set_error("cache_attention: %lld sequences of %lld key heads", (long long)sequences, (long long)kv_heads);
+      return -1;
+    }
+    TokenCall t{};
+    t.q = c.q, t.o = c.o, t.cache = c.cache, t.s = c.s, t.heads = c.heads, t.group = (int)(heads / kv_heads);
+    t.window = c.window, t.scale = c.scale;
+    launch_cache_tokens(kind == BF16, (int)d, t, p, workspace, (hipStream_t)stream);
+    return launched();
+  }
   const dim3 grid((unsigned)(tokens * heads));
 #define KRN_SIMPLE(BF, D) hipLaunchKernelGGL((cache_attention_simple<BF, D>), grid, dim3(64), 0, (hipStream_t)stream, c)
   if (kind == BF16 && d == 128) KRN_SIMPLE(true, 128);
@@ -123,10 +157,5 @@ extern "C" int krn_cache_attention(int kind, const void* q, const void* keys, co
   else if (d == 128) KRN_SIMPLE(false, 128);
   else KRN_SIMPLE(false, 64);
 #undef KRN_SIMPLE
-  hipError_t err = hipGetLastError();
-  if (err != hipSuccess) {
-    krn_set_error("cache_attention launch: %s", hipGetErrorString(err));
-    return (int)err;
-  }
-  return 0;
+  return launched();
 }

@@ -8,8 +8,7 @@ namespace krn {
 
 struct CacheView {
   const void *keys, *values;  // (pages, kv_heads, page, d) of 16-bit elements
-  int64_t pages;
-  int kv_heads, page_shift;   // a page holds 2^page_shift keys, 16 or more
+  int pages, kv_heads, page_shift;  // a page holds 2^page_shift keys, 16 or more
 };
 
 struct SequencesView {
@@ -32,6 +31,37 @@ __device__ __forceinline__ int sequence_length(const SequencesView& s, int i) { 
 __device__ __forceinline__ int held_keys(const SequencesView& s, int length, int page_shift) {
   return (int)min((int64_t)length, (int64_t)s.width << page_shift);
 }
+
+// The first key that a token at `position` sees through a window of that many keys (0: all)
+__device__ __forceinline__ int first_key(int position, int window) {
+  return window ? (int)max((int64_t)0, (int64_t)position + 1 - window) : 0;
+}
+
+// Attention of new tokens, a few of every sequence (cache_token.hip)
+constexpr int TOKEN_WAVES = 4;
+constexpr int TOKEN_ROWS = 64;     // rows of a key head, at most; more are a prompt's
+constexpr int TOKEN_PARTS = 2048;  // parts that the keys of all sequences and columns are shared out to
+constexpr int TOKEN_SPLIT = 2048;  // sequences; more keep the keys of each in one workgroup
+
+struct TokenCall {
+  const uint16_t* q;
+  uint16_t* o;
+  CacheView cache;
+  SequencesView s;
+  int heads, group, window;  // group: query heads of a key head
+  float scale;               // of the scores, times log2(e)
+  int rows, row_groups, kept, columns, split;  // of TokenPlan
+  int4* header;   // the number of split sequences, then of each (sequence, first slot, parts, -)
+  float* planes;  // a slot: of every column, `kept` rows of sums and their maxima and sums of weights
+};
+
+// rows: of a key head; blocks: of sixteen rows that a workgroup takes; kept: its rows; columns: key heads times groups of rows
+struct TokenPlan {
+  int64_t rows, blocks, row_groups, kept, columns, workgroups, joins, header_bytes, bytes;
+  bool split;
+};
+TokenPlan token_plan(int64_t step, int64_t group, int64_t kv_heads, int64_t d, int64_t page, int64_t sequences, int64_t width);
+void launch_cache_tokens(bool bf, int d, TokenCall c, const TokenPlan& p, void* workspace, hipStream_t stream);
 
 }  // namespace krn
 

@@ -1,0 +1,499 @@
+// Attention of a few new tokens a sequence over a paged cache: the rows of one key head (its query heads times the new tokens)
+// are multiplied with the head's keys and values, which are read once. What bounds it is that stream, so the keys of a
+// sequence are shared out over workgroups and joined by a second kernel.
+//
+// Shares. A tile is 32 keys. With T tiles in all sequences and C columns (key heads times groups of rows), a part has
+// at most chunk = max(4, T C / TOKEN_PARTS) tiles, one a wave at least, and sequence i is ceil(tiles_i / chunk) parts of
+// equal size: long and short sequences together keep every CU busy to the end. Only the device knows the lengths, so each
+// workgroup counts the parts before its own, one load a thread for 256 sequences.
+//
+// A wave computes S^T = K Q^T and O^T += V^T P^T with 16x16x32 MFMAs on its own tiles. A lane then holds one query row
+// (lane & 15) and eight keys of a tile: keys 4 g + r and 16 + 4 g + r, g = lane / 16, which are also the eight that it gives
+// the second product, so P goes from registers to registers. The maximum is exchanged between lanes only when a row exceeds the
+// running one by more than 2^8 in weight. P is kept in two 16-bit parts (2^-17 of a weight or less is left): the matrix cores
+// are idle nine tenths of the time.
+//
+// K and V tiles come into LDS by direct loads, one buffer each a wave and no barrier: K's next tile leaves when this one's
+// fragments are in registers, V's likewise, so 8 to 16 KiB a wave are always on their way. Sixteen keys lie in one page,
+// whose rows up to the sequence's end are a buffer resource: rows past it, and pages that are not there, read as zeros.
+#include "cache_parts.h"
+
+namespace krn {
+
+// the B operand's 16-bit parts and the products, by format
+template <bool BF>
+struct Narrow {
+  static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return f2bf2(lo, hi); }
+  static __device__ __forceinline__ float low(uint32_t w) { return __uint_as_float(w << 16); }
+  static __device__ __forceinline__ float high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+};
+template <>
+struct Narrow<false> {
+  static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return (uint32_t)f2h(lo) | ((uint32_t)f2h(hi) << 16); }
+  static __device__ __forceinline__ float low(uint32_t w) { return h2f((uint16_t)(w & 0xffff)); }
+  static __device__ __forceinline__ float high(uint32_t w) { return h2f((uint16_t)(w >> 16)); }
+};
+
+// The 16-byte chunk of a row that lies in slot `slot` of its row in LDS, so that reads of sixteen rows spread over the banks:
+// K's take one chunk of each row, V's transposed reads 32 bytes of each.
+template <int D>
+__device__ __forceinline__ int key_chunk(int row, int slot) {
+  return D == 128 ? slot ^ (row & 15) : slot ^ ((row >> 1) & 7);
+}
+template <int D>
+__device__ __forceinline__ int value_chunk(int row, int slot) {
+  return D == 128 ? slot ^ ((row & 7) << 1) : slot ^ (((row >> 1) & 3) << 1);
+}
+
+// fragments of both 16-key halves of a K tile: A operands, lane = key, 8 columns of step s
+template <int D>
+__device__ __forceinline__ void key_fragments(uint32_t at, u32x4 (&k)[2][D / 32]) {
+  if constexpr (D == 128) {
+    asm volatile(
+        "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %10\n\tds_read_b128 %3, %11\n\t"
+        "ds_read_b128 %4, %8 offset:4096\n\tds_read_b128 %5, %9 offset:4096\n\tds_read_b128 %6, %10 offset:4096\n\t"
+        "ds_read_b128 %7, %11 offset:4096\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(k[0][0]), "=&v"(k[0][1]), "=&v"(k[0][2]), "=&v"(k[0][3]), "=&v"(k[1][0]), "=&v"(k[1][1]), "=&v"(k[1][2]),
+          "=&v"(k[1][3])
+        : "v"(at), "v"(at ^ 64), "v"(at ^ 128), "v"(at ^ 192)
+        : "memory");
+  } else {
+    asm volatile(
+        "ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %4 offset:2048\n\tds_read_b128 %3, %5 offset:2048\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(k[0][0]), "=&v"(k[0][1]), "=&v"(k[1][0]), "=&v"(k[1][1])
+        : "v"(at), "v"(at ^ 64)
+        : "memory");
+  }
+}
+
+// V^T fragments of four blocks of 16 columns, each four keys of both halves
+template <int D>
+__device__ __forceinline__ void value_fragments(uint32_t at, u32x4 (&v)[4]) {
+  u32x2 w[8];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\tds_read_b64_tr_b16 %2, %9\n\t"
+      "ds_read_b64_tr_b16 %3, %9 offset:%12\n\tds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(w[4]), "=&v"(w[5]), "=&v"(w[6]), "=&v"(w[7])
+      : "v"(at), "v"(at ^ 32), "v"(at ^ 64), "v"(at ^ 96), "n"(16 * D * 2)
+      : "memory");
+#pragma unroll
+  for (int b = 0; b < 4; ++b) v[b] = u32x4{w[2 * b][0], w[2 * b][1], w[2 * b + 1][0], w[2 * b + 1][1]};
+}
+
+// the largest value of the four lanes that hold one row
+__device__ __forceinline__ float row_max(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float row_sum(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// The tiles of a sequence that its new tokens see: keys from the first one's window to the end
+struct TileRange {
+  int first, count;
+};
+__device__ __forceinline__ TileRange tiles_of(const TokenCall& c, int length) {
+  const int end = held_keys(c.s, length, c.cache.page_shift);
+  const int low = first_key(length - c.s.step, c.window);
+  const int first = low / 32;
+  return {first, low < end ? (end + 31) / 32 - first : 0};
+}
+
+// What a workgroup of column `c` number w does: part `part` of `parts` of sequence `seq`; a split sequence is the
+// `order`-th of them and its parts' sums go to slots from `slot` on.
+struct Share {
+  int seq, part, parts, slot, order;
+};
+
+// Counts of the parts before this workgroup's, packed: parts, parts of split sequences, split sequences
+constexpr int COUNT_BITS = 21;
+__device__ __forceinline__ uint64_t packed_parts(int parts) {
+  return (uint64_t)parts | (parts > 1 ? (uint64_t)parts << COUNT_BITS | (uint64_t)1 << (2 * COUNT_BITS) : 0);
+}
+constexpr uint64_t COUNT_MASK = (1 << COUNT_BITS) - 1;
+
+__device__ __forceinline__ uint64_t wave_scan(uint64_t x, int lane) {  // inclusive
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint64_t y = __shfl_up((unsigned long long)x, d);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+
+__device__ __forceinline__ bool find_share(const TokenCall& c, int w, bool first_column, Share& share) {
+  __shared__ uint64_t sums[8];
+  __shared__ Share found;
+  if (!c.split) {
+    share = {w, 0, 1, 0, 0};
+    return true;
+  }
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, per = (c.s.n + 255) / 256, begin = t * per;
+  if (t == 0) found.seq = -1;
+  uint64_t tiles = 0;
+  int one = 0;  // the tiles of this thread's first sequence
+  for (int k = 0; k < per && begin + k < c.s.n; ++k) {
+    const int count = tiles_of(c, sequence_length(c.s, begin + k)).count;
+    if (k == 0) one = count;
+    tiles += count;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) tiles += __shfl_xor((unsigned long long)tiles, d);
+  if (lane == 0) sums[wave] = tiles;
+  __syncthreads();
+  tiles = sums[0] + sums[1] + sums[2] + sums[3];
+  const uint64_t even = (tiles * c.columns + TOKEN_PARTS - 1) / TOKEN_PARTS;
+  const int chunk = (int)max((uint64_t)4, even);
+  const auto parts_of = [&](int count) { return max(1, (int)(((int64_t)count + chunk - 1) / chunk)); };
+  uint64_t mine = 0;
+  for (int k = 0; k < per && begin + k < c.s.n; ++k)
+    mine += packed_parts(parts_of(k == 0 ? one : tiles_of(c, sequence_length(c.s, begin + k)).count));
+  const uint64_t upto = wave_scan(mine, lane);
+  if (lane == 63) sums[4 + wave] = upto;
+  __syncthreads();
+  uint64_t before = upto - mine, all = 0;
+  for (int i = 0; i < 4; ++i) {
+    before += i < wave ? sums[4 + i] : 0;
+    all += sums[4 + i];
+  }
+  if ((int)(before & COUNT_MASK) <= w && w < (int)((before + mine) & COUNT_MASK)) {
+    for (int k = 0; k < per && begin + k < c.s.n; ++k) {
+      const int parts = parts_of(k == 0 ? one : tiles_of(c, sequence_length(c.s, begin + k)).count);
+      const int at = (int)(before & COUNT_MASK);
+      if (w < at + parts) {
+        found = {begin + k, w - at, parts, (int)(before >> COUNT_BITS & COUNT_MASK), (int)(before >> (2 * COUNT_BITS))};
+        break;
+      }
+      before += packed_parts(parts);
+    }
+  }
+  if (first_column && w == 0 && t == 0) c.header[0] = {(int)(all >> (2 * COUNT_BITS)), 0, 0, 0};
+  __syncthreads();
+  share = found;
+  return share.seq >= 0;
+}
+
+template <bool BF, int D, int NB>
+__global__ __launch_bounds__(64 * TOKEN_WAVES, NB < 4 ? 2 : 1) void cache_tokens(TokenCall c) {
+  constexpr int RB = D * 2, DCH = D / 8, HALF = 16 * RB, TILE = 2 * HALF, LOADS = HALF / 1024, ROWS = 16 * NB;
+  constexpr int OLD = D + 4;  // floats per row of a wave's O in LDS
+  static_assert(16 * OLD * 4 <= 2 * TILE, "a wave's rows fit its buffers");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[TOKEN_WAVES * 2 * TILE];
+  __shared__ float stat[2][TOKEN_WAVES][16];
+  const int w = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / c.columns)), column = (int)blockIdx.x - w * c.columns;
+  Share share;
+  if (!find_share(c, w, column == 0, share)) return;
+  const int seq = __builtin_amdgcn_readfirstlane(share.seq), part = __builtin_amdgcn_readfirstlane(share.part),
+            parts = __builtin_amdgcn_readfirstlane(share.parts), slot = __builtin_amdgcn_readfirstlane(share.slot);
+  const int t = threadIdx.x, lane = t & 63, g = lane >> 4, col = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  if (parts > 1 && part == 0 && column == 0 && t == 0) c.header[1 + share.order] = {seq, slot, parts, 0};
+
+  const int kv = __builtin_amdgcn_readfirstlane(column / c.row_groups), row0 = (column - kv * c.row_groups) * ROWS, rows = min(ROWS, c.rows - row0);
+  const int length = __builtin_amdgcn_readfirstlane(sequence_length(c.s, seq)), end = held_keys(c.s, length, c.cache.page_shift);
+  const TileRange range = tiles_of(c, length);
+  // the part's tiles and this wave's (below 2^26), in scalar registers, where a division leaves none
+  const int even = __builtin_amdgcn_readfirstlane(range.count / parts), over = range.count - even * parts;
+  const int begin = range.first + even * part + min(part, over), count = even + (part < over ? 1 : 0);
+  const int first = begin + count * wave / TOKEN_WAVES, last = begin + count * (wave + 1) / TOKEN_WAVES;
+
+  // queries as B operands (lane = row, 8 columns of step s) and the keys that each row sees, [low, limit)
+  u32x4 qf[NB][D / 32];
+  int limit[NB], low[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int r = row0 + b * 16 + col, j = r / c.group;
+    const bool real = r < c.rows;
+    const uint16_t* q = c.q + (((int64_t)seq * c.s.step + j) * c.heads + kv * c.group + (r - j * c.group)) * D;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) qf[b][s] = real ? *reinterpret_cast<const u32x4*>(q + s * 32 + g * 8) : u32x4{};
+    const int position = length - c.s.step + j;
+    limit[b] = real ? min(position + 1, end) : end;
+    low[b] = real ? first_key(position, c.window) : 0;
+  }
+  // tiles in these bounds have no masked key
+  const int all_low = first_key(length - 1, c.window), all_limit = min(length - c.s.step + 1, end);
+
+  uint8_t *kbuf = lds + wave * 2 * TILE, *vbuf = kbuf + TILE;
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)kbuf;
+  const uint32_t kat = lds_at + col * RB + key_chunk<D>(col, g) * 16;
+  const int vrow = g * 4 + (col >> 2);
+  const uint32_t vat = lds_at + TILE + vrow * RB + value_chunk<D>(vrow, 0) * 16 + (col & 3) * 8;
+  uint32_t koff[LOADS], voff[LOADS];  // byte offsets within sixteen keys
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) {
+    const int row = j * (1024 / RB) + lane / DCH, s = lane % DCH;
+    koff[j] = (uint32_t)(row * RB + key_chunk<D>(row, s) * 16);
+    voff[j] = (uint32_t)(row * RB + value_chunk<D>(row, s) * 16);
+  }
+
+  // page numbers of 64 groups of sixteen keys, a lane each
+  const int* table = c.s.table + (int64_t)seq * c.s.width;
+  const int shift = c.cache.page_shift;
+  int ids = -1, ids_from = 0;
+  const auto fetch_ids = [&](int tile) {
+    ids_from = tile * 2;
+    const int64_t at = ((int64_t)(ids_from + lane) * 16) >> shift;
+    ids = at < c.s.width ? table[at] : -1;
+    asm volatile("" : "+v"(ids));  // waited for here: a use in the loop would wait for the tiles on their way each time
+  };
+  // the rows of sixteen keys from key0 on: where they start and how many bytes the sequence has there
+  struct Group {
+    int64_t at;
+    int bytes;
+  };
+  const auto group_of = [&](int tile, int h) {
+    const int number = __builtin_amdgcn_readlane(ids, tile * 2 + h - ids_from), key0 = tile * 32 + h * 16;
+    const bool there = (uint32_t)number < (uint32_t)c.cache.pages;
+    const int64_t row = ((((int64_t)(there ? number : 0) * c.cache.kv_heads + kv) << shift) + (key0 & ((1 << shift) - 1)));
+    return Group{row * RB, __builtin_amdgcn_readfirstlane(there ? max(0, min(16, end - key0)) * RB : 0)};
+  };
+  Group now[2];  // of the tile whose V is next
+  const auto load_keys = [&](int tile) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      now[h] = group_of(tile, h);
+      const __amdgpu_buffer_rsrc_t r = panel_rsrc((const uint8_t*)c.cache.keys + now[h].at, now[h].bytes);
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) buffer_to_lds16(r, kbuf + h * HALF + j * 1024, koff[j], 0);
+    }
+  };
+  const auto load_values = [&]() {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const __amdgpu_buffer_rsrc_t r = panel_rsrc((const uint8_t*)c.cache.values + now[h].at, now[h].bytes);
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) buffer_to_lds16(r, vbuf + h * HALF + j * 1024, voff[j], 0);
+    }
+  };
+
+  f32x4 acc[NB][D / 16];
+  float m[NB], base[NB], total[NB];  // base: m, or 0 while no key has been seen
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    m[b] = -INFINITY, base[b] = 0.0f, total[b] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) acc[b][i] = f32x4{};
+  }
+  if (first < last) {
+    fetch_ids(first);
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s) asm volatile("" : "+v"(qf[b][s]));  // here too, for the same reason
+    load_keys(first);
+    load_values();
+  }
+  for (int tile = first; tile < last; ++tile) {
+    const bool more = tile + 1 < last;
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory");  // K is here, V may be on its way
+    u32x4 kf[2][D / 32];
+    key_fragments<D>(kat, kf);
+    if (more) {
+      if ((tile + 1) * 2 - ids_from >= 64) fetch_ids(tile + 1);
+      load_keys(tile + 1);
+    }
+    u32x4 ph[NB], pl[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      f32x4 s[2] = {};
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) s[h] = Narrow<BF>::mma(kf[h][i], qf[b][i], s[h]);
+      float x[8], top = -INFINITY;
+      const int key = tile * 32 + g * 4;
+      const bool masked = tile * 32 < all_low || tile * 32 + 32 > all_limit;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3] * c.scale;
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int k = key + (e >> 2) * 16 + (e & 3);
+          if (k >= limit[b] || k < low[b]) x[e] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);
+      // the base moves only when a weight would exceed 2^8: then maxima meet, and acc and total are rescaled
+      if (__builtin_amdgcn_ballot_w64(top > m[b] + 8.0f) != 0) {
+        const float next = fmaxf(m[b], row_max(top)), to_base = next == -INFINITY ? 0.0f : next;
+        const float corr = __builtin_amdgcn_exp2f(m[b] - to_base);
+        total[b] *= corr;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) acc[b][i] *= corr;
+        m[b] = next, base[b] = to_base;
+      }
+      float sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = __builtin_amdgcn_exp2f(x[2 * e] - base[b]), p1 = __builtin_amdgcn_exp2f(x[2 * e + 1] - base[b]);
+        sum += p0 + p1;
+        ph[b][e] = Narrow<BF>::pack(p0, p1);
+        pl[b][e] = Narrow<BF>::pack(p0 - Narrow<BF>::low(ph[b][e]), p1 - Narrow<BF>::high(ph[b][e]));
+      }
+      total[b] += sum;
+    }
+    if (more)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory");  // V is here, the next K may be on its way
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int q = 0; q < D / 64; ++q) {
+      u32x4 vf[4];
+      value_fragments<D>(vat ^ (q * 128), vf);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          acc[b][q * 4 + i] = Narrow<BF>::mma(vf[i], ph[b], acc[b][q * 4 + i]);
+          acc[b][q * 4 + i] = Narrow<BF>::mma(vf[i], pl[b], acc[b][q * 4 + i]);
+        }
+    }
+    if (more) load_values();
+  }
+
+  // the waves' rows meet in LDS, sixteen at a time: a lane has columns i * 16 + 4 g to + 3 of its row
+  float* mine = reinterpret_cast<float*>(kbuf);
+  float* plane = c.planes + ((int64_t)slot + part) * c.columns * c.kept * (D + 4) + (int64_t)column * c.kept * (D + 4);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    if (b * 16 >= rows) break;
+    const float sum = row_sum(total[b]);
+    __syncthreads();  // every wave is done with its tiles, or with the rows before
+    if (g == 0) stat[0][wave][col] = m[b], stat[1][wave][col] = sum;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(mine + col * OLD + i * 16 + g * 4) = acc[b][i];
+    __syncthreads();
+    for (int at = t; at < min(16, rows - b * 16) * (D / 4); at += 64 * TOKEN_WAVES) {
+      const int row = at / (D / 4), d = at % (D / 4) * 4;
+      float top = stat[0][0][row];
+#pragma unroll
+      for (int x = 1; x < TOKEN_WAVES; ++x) top = fmaxf(top, stat[0][x][row]);
+      const float to_base = top == -INFINITY ? 0.0f : top;
+      float all = 0.0f;
+      f32x4 o = f32x4{};
+#pragma unroll
+      for (int x = 0; x < TOKEN_WAVES; ++x) {
+        const float f = __builtin_amdgcn_exp2f(stat[0][x][row] - to_base);
+        all += f * stat[1][x][row];
+        o += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * 2 * TILE) + row * OLD + d);
+      }
+      if (parts > 1) {  // unnormalised rows, then their maxima and sums
+        const int r = b * 16 + row;
+        *reinterpret_cast<f32x4*>(plane + r * D + d) = o;
+        if (d == 0) plane[c.kept * D + r * 2] = top, plane[c.kept * D + r * 2 + 1] = all;
+      } else {
+        const int r = row0 + b * 16 + row, j = r / c.group;
+        const float inv = all == 0.0f ? 0.0f : 1.0f / all;  // no key: zeros
+        const u32x2 y = {Narrow<BF>::pack(o[0] * inv, o[1] * inv), Narrow<BF>::pack(o[2] * inv, o[3] * inv)};
+        *reinterpret_cast<u32x2*>(c.o + (((int64_t)seq * c.s.step + j) * c.heads + kv * c.group + (r - j * c.group)) * D + d) = y;
+      }
+    }
+  }
+}
+
+// One row of a split sequence from its parts: JOIN_THREADS / (D / 4) parts side by side, four columns a thread
+constexpr int JOIN_THREADS = 512;
+template <bool BF, int D>
+__global__ __launch_bounds__(JOIN_THREADS) void cache_join(TokenCall c) {
+  constexpr int LANES = JOIN_THREADS / (D / 4);
+  __shared__ f32x4 sums[LANES][D / 4];
+  __shared__ float stat[2][LANES];
+  const int rest = (int)(blockIdx.x / c.columns), column = (int)(blockIdx.x % c.columns), order = rest / c.kept, r = rest % c.kept;
+  if (order >= c.header[0].x) return;
+  const int4 head = c.header[1 + order];
+  const int kv = column / c.row_groups, row = column % c.row_groups * c.kept + r;
+  if (row >= c.rows) return;
+  const int t = threadIdx.x, side = t / (D / 4), d = t % (D / 4) * 4;
+  const int64_t stride = (int64_t)c.columns * c.kept * (D + 4);
+  const float* plane = c.planes + head.y * stride + (int64_t)column * c.kept * (D + 4);
+  float m = -INFINITY, total = 0.0f;
+  f32x4 o = f32x4{};
+#pragma unroll 4
+  for (int p = side; p < head.z; p += LANES) {
+    const float* at = plane + p * stride;
+    const float top = at[c.kept * D + r * 2], sum = at[c.kept * D + r * 2 + 1], next = fmaxf(m, top);
+    const float to_base = next == -INFINITY ? 0.0f : next;
+    const float f = __builtin_amdgcn_exp2f(m - to_base), h = __builtin_amdgcn_exp2f(top - to_base);
+    total = total * f + sum * h;
+    o = o * f + h * *reinterpret_cast<const f32x4*>(at + r * D + d);
+    m = next;
+  }
+  sums[side][d / 4] = o;
+  if (d == 0) stat[0][side] = m, stat[1][side] = total;
+  __syncthreads();
+  if (side != 0) return;
+  float top = stat[0][0];
+#pragma unroll
+  for (int x = 1; x < LANES; ++x) top = fmaxf(top, stat[0][x]);
+  const float to_base = top == -INFINITY ? 0.0f : top;
+  float all = 0.0f;
+  o = f32x4{};
+#pragma unroll
+  for (int x = 0; x < LANES; ++x) {
+    const float f = __builtin_amdgcn_exp2f(stat[0][x] - to_base);
+    all += f * stat[1][x];
+    o += f * sums[x][d / 4];
+  }
+  const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+  const int j = row / c.group;
+  const u32x2 y = {Narrow<BF>::pack(o[0] * inv, o[1] * inv), Narrow<BF>::pack(o[2] * inv, o[3] * inv)};
+  *reinterpret_cast<u32x2*>(c.o + (((int64_t)head.x * c.s.step + j) * c.heads + kv * c.group + (row - j * c.group)) * D + d) = y;
+}
+
+}  // namespace krn
+
+using namespace krn;
+
+TokenPlan krn::token_plan(int64_t step, int64_t group, int64_t kv_heads, int64_t d, int64_t page, int64_t sequences, int64_t width) {
+  TokenPlan p{};
+  p.rows = step * group;
+  p.blocks = p.rows <= 16 ? 1 : p.rows <= 32 ? 2 : 4;
+  p.row_groups = (p.rows + 16 * p.blocks - 1) / (16 * p.blocks);
+  p.kept = p.rows < 16 * p.blocks ? p.rows : 16 * p.blocks;
+  p.columns = kv_heads * p.row_groups;
+  const int64_t tiles = (width * page < 0x7fffffff ? width * page : 0x7fffffff) / 32 + 1;  // of a sequence, at most
+  // parts beyond the first of all sequences: no more than TOKEN_PARTS by the size of a part, nor than a part has tiles
+  int64_t extra = TOKEN_PARTS / p.columns;
+  if (sequences * ((tiles - 1) / 4) < extra) extra = sequences * ((tiles - 1) / 4);
+  if (sequences > TOKEN_SPLIT) extra = 0;
+  p.workgroups = sequences + extra;
+  p.split = extra > 0;
+  p.joins = sequences < extra ? sequences : extra;
+  p.header_bytes = p.split ? (p.joins + 1) * 16 : 0;
+  // a split sequence has at most twice as many parts as beyond its first
+  p.bytes = p.split ? p.header_bytes + 2 * extra * p.columns * p.kept * (d + 4) * 4 : 0;
+  return p;
+}
+
+template <bool BF, int D>
+static void launch(const TokenCall& c, const TokenPlan& p, hipStream_t stream) {
+  const dim3 grid((unsigned)(p.workgroups * p.columns)), block(64 * TOKEN_WAVES);
+  if (p.blocks == 1) hipLaunchKernelGGL((cache_tokens<BF, D, 1>), grid, block, 0, stream, c);
+  else if (p.blocks == 2) hipLaunchKernelGGL((cache_tokens<BF, D, 2>), grid, block, 0, stream, c);
+  else hipLaunchKernelGGL((cache_tokens<BF, D, 4>), grid, block, 0, stream, c);
+  if (c.split)
+    hipLaunchKernelGGL((cache_join<BF, D>), dim3((unsigned)(p.joins * p.kept * p.columns)), dim3(JOIN_THREADS), 0, stream, c);
+}
+
+void krn::launch_cache_tokens(bool bf, int d, TokenCall c, const TokenPlan& p, void* workspace, hipStream_t stream) {
+  c.rows = (int)p.rows, c.row_groups = (int)p.row_groups, c.kept = (int)p.kept, c.columns = (int)p.columns, c.split = p.split;
+  c.header = (int4*)workspace, c.planes = (float*)((char*)workspace + p.header_bytes);
+  if (bf) d == 128 ? launch<true, 128>(c, p, stream) : launch<true, 64>(c, p, stream);
+  else d == 128 ? launch<false, 128>(c, p, stream) : launch<false, 64>(c, p, stream);
+}

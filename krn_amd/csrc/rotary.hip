@@ -226,7 +226,7 @@ bool krn_cache_arguments(const CacheArguments& a, CacheView& cache, SequencesVie
   }
   int shift = 4;
   while ((1 << shift) < a.page) ++shift;
-  cache = {a.keys, a.values, a.pages, (int)a.kv_heads, shift};
+  cache = {a.keys, a.values, (int)a.pages, (int)a.kv_heads, shift};
   sequences = {(const int*)a.starts, (const int*)a.lengths, (const int*)a.table, (int)a.sequences,
                (int)a.width, a.starts ? 0 : (int)a.step, (int)a.tokens};
   return true;
