@@ -40,8 +40,11 @@ __device__ __forceinline__ int first_key(int position, int window) {
 // Attention of new tokens, a few of every sequence (cache_token.hip)
 constexpr int TOKEN_WAVES = 4;
 constexpr int TOKEN_ROWS = 64;     // rows of a key head, at most; more are a prompt's
-constexpr int TOKEN_PARTS = 2048;  // parts that the keys of all sequences and columns are shared out to
+constexpr int TOKEN_PARTS = 1024;  // parts that the keys of all sequences and columns are shared out to
+constexpr int TOKEN_CHUNK = 4;     // tiles of a part, at least
 constexpr int TOKEN_SPLIT = 2048;  // sequences; more keep the keys of each in one workgroup
+constexpr int TOKEN_TILES = 1 << 20;  // of a sequence, as far as shares go by them: the sum of all stays below 2^32
+static_assert(TOKEN_PARTS + TOKEN_SPLIT < 1 << 16, "parts are counted in 16 bits");
 
 struct TokenCall {
   const uint16_t* q;
@@ -51,13 +54,14 @@ struct TokenCall {
   int heads, group, window;  // group: query heads of a key head
   float scale;               // of the scores, times log2(e)
   int rows, row_groups, kept, columns, split;  // of TokenPlan
-  int4* header;   // the number of split sequences, then of each (sequence, first slot, parts, -)
-  float* planes;  // a slot: of every column, `kept` rows of sums and their maxima and sums of weights
+  uint32_t shares;  // the parts of a column, with all sequences in one row
+  int4* header;     // the number of sequences in several parts, then of each (sequence, first workgroup, parts, -)
+  float* planes;    // of a workgroup and column: `kept` rows of sums, then their maxima and sums of weights
 };
 
 // rows: of a key head; blocks: of sixteen rows that a workgroup takes; kept: its rows; columns: key heads times groups of rows
 struct TokenPlan {
-  int64_t rows, blocks, row_groups, kept, columns, workgroups, joins, header_bytes, bytes;
+  int64_t rows, blocks, row_groups, kept, columns, shares, workgroups, joins, header_bytes, bytes;
   bool split;
 };
 TokenPlan token_plan(int64_t step, int64_t group, int64_t kv_heads, int64_t d, int64_t page, int64_t sequences, int64_t width);

@@ -3,9 +3,9 @@
 // sequence are shared out over workgroups and joined by a second kernel.
 //
 // Shares. A tile is 32 keys. With T tiles in all sequences and C columns (key heads times groups of rows), a part has
-// at most chunk = max(4, T C / TOKEN_PARTS) tiles, one a wave at least, and sequence i is ceil(tiles_i / chunk) parts of
-// equal size: long and short sequences together keep every CU busy to the end. Only the device knows the lengths, so each
-// workgroup counts the parts before its own, one load a thread for 256 sequences.
+// at most chunk = max(TOKEN_CHUNK, T C / TOKEN_PARTS) tiles, and sequence i is ceil(tiles_i / chunk) parts of equal size:
+// long and short sequences together keep every CU busy to the end. Only the device knows the lengths, so each wave
+// counts the parts before its own.
 //
 // A wave computes S^T = K Q^T and O^T += V^T P^T with 16x16x32 MFMAs on its own tiles. A lane then holds one query row
 // (lane & 15) and eight keys of a tile: keys 4 g + r and 16 + 4 g + r, g = lane / 16, which are also the eight that it gives
@@ -113,78 +113,73 @@ __device__ __forceinline__ TileRange tiles_of(const TokenCall& c, int length) {
   return {first, low < end ? (end + 31) / 32 - first : 0};
 }
 
-// What a workgroup of column `c` number w does: part `part` of `parts` of sequence `seq`; a split sequence is the
-// `order`-th of them and its parts' sums go to slots from `slot` on.
+// What workgroup w of a column does: part `part` of `parts` of sequence `seq`, the `order`-th of those in several parts
 struct Share {
-  int seq, part, parts, slot, order;
+  int seq, part, parts, order;
 };
 
-// Counts of the parts before this workgroup's, packed: parts, parts of split sequences, split sequences
-constexpr int COUNT_BITS = 21;
-__device__ __forceinline__ uint64_t packed_parts(int parts) {
-  return (uint64_t)parts | (parts > 1 ? (uint64_t)parts << COUNT_BITS | (uint64_t)1 << (2 * COUNT_BITS) : 0);
+// the sum over lanes up to this one: rows of sixteen by shifts, then the rows' ends
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t from_lane(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
 }
-constexpr uint64_t COUNT_MASK = (1 << COUNT_BITS) - 1;
-
-__device__ __forceinline__ uint64_t wave_scan(uint64_t x, int lane) {  // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint64_t y = __shfl_up((unsigned long long)x, d);
-    if (lane >= d) x += y;
-  }
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x += from_lane<0x111, 0xf>(x);
+  x += from_lane<0x112, 0xf>(x);
+  x += from_lane<0x114, 0xf>(x);
+  x += from_lane<0x118, 0xf>(x);
+  x += from_lane<0x142, 0xa>(x);  // lane 15 to the second row, lane 47 to the fourth
+  x += from_lane<0x143, 0xc>(x);  // lane 31 to the upper half
   return x;
 }
 
-__device__ __forceinline__ bool find_share(const TokenCall& c, int w, bool first_column, Share& share) {
-  __shared__ uint64_t sums[8];
-  __shared__ Share found;
+// Every wave counts for itself, a lane for ceil(n / 64) sequences in a row, so that no barrier is needed.
+__device__ __forceinline__ bool find_share(const TokenCall& c, int w, bool writes, Share& share) {
   if (!c.split) {
-    share = {w, 0, 1, 0, 0};
+    share = {w, 0, 1, 0};
     return true;
   }
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, per = (c.s.n + 255) / 256, begin = t * per;
-  if (t == 0) found.seq = -1;
-  uint64_t tiles = 0;
-  int one = 0;  // the tiles of this thread's first sequence
-  for (int k = 0; k < per && begin + k < c.s.n; ++k) {
-    const int count = tiles_of(c, sequence_length(c.s, begin + k)).count;
-    if (k == 0) one = count;
-    tiles += count;
-  }
+  constexpr int HELD = 4;  // sequences a lane keeps in registers
+  const int lane = threadIdx.x & 63, per = (c.s.n + 63) / 64, first = lane * per, mine = max(0, min(per, c.s.n - first));
+  const auto weight_of = [&](int i) { return (uint32_t)min(tiles_of(c, sequence_length(c.s, i)).count, TOKEN_TILES); };
+  uint32_t held[HELD], tiles = 0;
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) tiles += __shfl_xor((unsigned long long)tiles, d);
-  if (lane == 0) sums[wave] = tiles;
-  __syncthreads();
-  tiles = sums[0] + sums[1] + sums[2] + sums[3];
-  const uint64_t even = (tiles * c.columns + TOKEN_PARTS - 1) / TOKEN_PARTS;
-  const int chunk = (int)max((uint64_t)4, even);
-  const auto parts_of = [&](int count) { return max(1, (int)(((int64_t)count + chunk - 1) / chunk)); };
-  uint64_t mine = 0;
-  for (int k = 0; k < per && begin + k < c.s.n; ++k)
-    mine += packed_parts(parts_of(k == 0 ? one : tiles_of(c, sequence_length(c.s, begin + k)).count));
-  const uint64_t upto = wave_scan(mine, lane);
-  if (lane == 63) sums[4 + wave] = upto;
-  __syncthreads();
-  uint64_t before = upto - mine, all = 0;
-  for (int i = 0; i < 4; ++i) {
-    before += i < wave ? sums[4 + i] : 0;
-    all += sums[4 + i];
+  for (int k = 0; k < HELD; ++k) {
+    held[k] = k < mine ? weight_of(first + k) : 0;
+    tiles += held[k];
   }
-  if ((int)(before & COUNT_MASK) <= w && w < (int)((before + mine) & COUNT_MASK)) {
-    for (int k = 0; k < per && begin + k < c.s.n; ++k) {
-      const int parts = parts_of(k == 0 ? one : tiles_of(c, sequence_length(c.s, begin + k)).count);
-      const int at = (int)(before & COUNT_MASK);
-      if (w < at + parts) {
-        found = {begin + k, w - at, parts, (int)(before >> COUNT_BITS & COUNT_MASK), (int)(before >> (2 * COUNT_BITS))};
-        break;
-      }
-      before += packed_parts(parts);
+  for (int k = HELD; k < mine; ++k) tiles += weight_of(first + k);
+  tiles = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(tiles), 63);
+  const uint32_t chunk = max((uint32_t)TOKEN_CHUNK, (tiles + c.shares - 1) / c.shares);
+  // parts in the low half, sequences of several in the high one
+  const auto parts_of = [&](uint32_t weight) { return max(1u, (weight + chunk - 1) / chunk); };
+  const auto packed = [&](uint32_t parts) { return parts + (parts > 1 ? 0x10000u : 0u); };
+  uint32_t count = 0;
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) {
+    held[k] = k < mine ? parts_of(held[k]) : 0;
+    count += packed(held[k]);
+  }
+  for (int k = HELD; k < mine; ++k) count += packed(parts_of(weight_of(first + k)));
+  const uint32_t upto = wave_scan(count), all = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+  if (writes && w == 0 && threadIdx.x == 0) c.header[0] = {(int)(all >> 16), 0, 0, 0};
+  uint32_t before = upto - count;
+  const uint64_t owner = __builtin_amdgcn_ballot_w64((int)(before & 0xffff) <= w && w < (int)(upto & 0xffff));
+  if (owner == 0) return false;
+  int seq = first, parts = 1;
+  for (int k = 0; k < mine; ++k) {  // in the owner's lane: its sequence
+    parts = k < HELD ? (int)(k == 0 ? held[0] : k == 1 ? held[1] : k == 2 ? held[2] : held[3]) : (int)parts_of(weight_of(first + k));
+    if (w < (int)(before & 0xffff) + parts) {
+      seq = first + k;
+      break;
     }
+    before += packed((uint32_t)parts);
   }
-  if (first_column && w == 0 && t == 0) c.header[0] = {(int)(all >> (2 * COUNT_BITS)), 0, 0, 0};
-  __syncthreads();
-  share = found;
-  return share.seq >= 0;
+  const int from = __builtin_ctzll(owner);
+  share.seq = __builtin_amdgcn_readlane(seq, from), share.parts = __builtin_amdgcn_readlane(parts, from);
+  before = (uint32_t)__builtin_amdgcn_readlane((int)before, from);
+  share.part = w - (int)(before & 0xffff), share.order = (int)(before >> 16);
+  return true;
 }
 
 template <bool BF, int D, int NB>
@@ -197,11 +192,10 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES, NB < 4 ? 2 : 1) void cache_tokens
   const int w = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / c.columns)), column = (int)blockIdx.x - w * c.columns;
   Share share;
   if (!find_share(c, w, column == 0, share)) return;
-  const int seq = __builtin_amdgcn_readfirstlane(share.seq), part = __builtin_amdgcn_readfirstlane(share.part),
-            parts = __builtin_amdgcn_readfirstlane(share.parts), slot = __builtin_amdgcn_readfirstlane(share.slot);
+  const int seq = share.seq, part = share.part, parts = share.parts;
   const int t = threadIdx.x, lane = t & 63, g = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  if (parts > 1 && part == 0 && column == 0 && t == 0) c.header[1 + share.order] = {seq, slot, parts, 0};
+  if (parts > 1 && part == 0 && column == 0 && t == 0) c.header[1 + share.order] = {seq, w, parts, 0};
 
   const int kv = __builtin_amdgcn_readfirstlane(column / c.row_groups), row0 = (column - kv * c.row_groups) * ROWS, rows = min(ROWS, c.rows - row0);
   const int length = __builtin_amdgcn_readfirstlane(sequence_length(c.s, seq)), end = held_keys(c.s, length, c.cache.page_shift);
@@ -269,7 +263,7 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES, NB < 4 ? 2 : 1) void cache_tokens
       now[h] = group_of(tile, h);
       const __amdgpu_buffer_rsrc_t r = panel_rsrc((const uint8_t*)c.cache.keys + now[h].at, now[h].bytes);
 #pragma unroll
-      for (int j = 0; j < LOADS; ++j) buffer_to_lds16(r, kbuf + h * HALF + j * 1024, koff[j], 0);
+      for (int j = 0; j < LOADS; ++j) buffer_to_lds16<true>(r, kbuf + h * HALF + j * 1024, koff[j], 0);
     }
   };
   const auto load_values = [&]() {
@@ -277,7 +271,7 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES, NB < 4 ? 2 : 1) void cache_tokens
     for (int h = 0; h < 2; ++h) {
       const __amdgpu_buffer_rsrc_t r = panel_rsrc((const uint8_t*)c.cache.values + now[h].at, now[h].bytes);
 #pragma unroll
-      for (int j = 0; j < LOADS; ++j) buffer_to_lds16(r, vbuf + h * HALF + j * 1024, voff[j], 0);
+      for (int j = 0; j < LOADS; ++j) buffer_to_lds16<true>(r, vbuf + h * HALF + j * 1024, voff[j], 0);
     }
   };
 
@@ -369,7 +363,7 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES, NB < 4 ? 2 : 1) void cache_tokens
 
   // the waves' rows meet in LDS, sixteen at a time: a lane has columns i * 16 + 4 g to + 3 of its row
   float* mine = reinterpret_cast<float*>(kbuf);
-  float* plane = c.planes + ((int64_t)slot + part) * c.columns * c.kept * (D + 4) + (int64_t)column * c.kept * (D + 4);
+  float* plane = c.planes + ((int64_t)w * c.columns + column) * c.kept * (D + 4);
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     if (b * 16 >= rows) break;
@@ -468,16 +462,16 @@ TokenPlan krn::token_plan(int64_t step, int64_t group, int64_t kv_heads, int64_t
   p.kept = p.rows < 16 * p.blocks ? p.rows : 16 * p.blocks;
   p.columns = kv_heads * p.row_groups;
   const int64_t tiles = (width * page < 0x7fffffff ? width * page : 0x7fffffff) / 32 + 1;  // of a sequence, at most
-  // parts beyond the first of all sequences: no more than TOKEN_PARTS by the size of a part, nor than a part has tiles
-  int64_t extra = TOKEN_PARTS / p.columns;
-  if (sequences * ((tiles - 1) / 4) < extra) extra = sequences * ((tiles - 1) / 4);
+  // parts beyond the first of all sequences, in each column: no more than shares, nor than parts have tiles
+  p.shares = TOKEN_PARTS / p.columns;
+  int64_t extra = p.shares;
+  if (sequences * ((tiles - 1) / TOKEN_CHUNK) < extra) extra = sequences * ((tiles - 1) / TOKEN_CHUNK);
   if (sequences > TOKEN_SPLIT) extra = 0;
   p.workgroups = sequences + extra;
   p.split = extra > 0;
   p.joins = sequences < extra ? sequences : extra;
   p.header_bytes = p.split ? (p.joins + 1) * 16 : 0;
-  // a split sequence has at most twice as many parts as beyond its first
-  p.bytes = p.split ? p.header_bytes + 2 * extra * p.columns * p.kept * (d + 4) * 4 : 0;
+  p.bytes = p.split ? p.header_bytes + p.workgroups * p.columns * p.kept * (d + 4) * 4 : 0;
   return p;
 }
 
@@ -493,6 +487,7 @@ static void launch(const TokenCall& c, const TokenPlan& p, hipStream_t stream) {
 
 void krn::launch_cache_tokens(bool bf, int d, TokenCall c, const TokenPlan& p, void* workspace, hipStream_t stream) {
   c.rows = (int)p.rows, c.row_groups = (int)p.row_groups, c.kept = (int)p.kept, c.columns = (int)p.columns, c.split = p.split;
+  c.shares = (uint32_t)p.shares;
   c.header = (int4*)workspace, c.planes = (float*)((char*)workspace + p.header_bytes);
   if (bf) d == 128 ? launch<true, 128>(c, p, stream) : launch<true, 64>(c, p, stream);
   else d == 128 ? launch<false, 128>(c, p, stream) : launch<false, 64>(c, p, stream);
