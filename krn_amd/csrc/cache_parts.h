@@ -67,6 +67,21 @@ struct TokenPlan {
 TokenPlan token_plan(int64_t step, int64_t group, int64_t kv_heads, int64_t d, int64_t page, int64_t sequences, int64_t width);
 void launch_cache_tokens(bool bf, int d, TokenCall c, const TokenPlan& p, void* workspace, hipStream_t stream);
 
+// Attention of packed prompts (cache_prompt.hip)
+constexpr int PROMPT_ROWS = 256;  // of a workgroup: tokens times query heads of a key head
+
+struct PromptCall {
+  const uint16_t* q;
+  uint16_t* o;
+  CacheView cache;
+  SequencesView s;
+  int heads, kv_heads, group, window, slots;  // group: query heads of a key head
+  float scale;                                // of the scores, times log2(e)
+};
+// Workgroups of a key head: without starts those of `step` tokens a sequence, else enough for any lengths (step 0)
+int64_t prompt_slots(int64_t tokens, int64_t step, int64_t group, int64_t sequences);
+void launch_cache_prompt(bool bf, int d, const PromptCall& c, hipStream_t stream);
+
 }  // namespace krn
 
 // Host side: what every entry point on a cache checks; false leaves a message.
