@@ -60,102 +60,20 @@ __device__ __forceinline__ bool find_tile(const PromptCall& c, int slot, PromptT
   return at >= 0 && (int64_t)at * PROMPT_ROWS < (int64_t)tile.range.count * c.group;
 }
 
-// V^T fragments of a tile: [step][block of 32 columns], a lane the keys of its P and one column. One assembly block with
-// its wait: as builtins the compiler waits for the tiles on their way before the first of them.
-template <int D>
-__device__ __forceinline__ void value_tile(uint32_t at, u32x4 (&v)[4][D / 32]) {
-  u32x2 w[4 * (D / 32) * 2];
-  if constexpr (D == 128) {
-    asm volatile(
-        "ds_read_b64_tr_b16 %0, %32\n\t"
-        "ds_read_b64_tr_b16 %1, %32 offset:2048\n\t"
-        "ds_read_b64_tr_b16 %2, %33\n\t"
-        "ds_read_b64_tr_b16 %3, %33 offset:2048\n\t"
-        "ds_read_b64_tr_b16 %4, %34\n\t"
-        "ds_read_b64_tr_b16 %5, %34 offset:2048\n\t"
-        "ds_read_b64_tr_b16 %6, %35\n\t"
-        "ds_read_b64_tr_b16 %7, %35 offset:2048\n\t"
-        "ds_read_b64_tr_b16 %8, %32 offset:4096\n\t"
-        "ds_read_b64_tr_b16 %9, %32 offset:6144\n\t"
-        "ds_read_b64_tr_b16 %10, %33 offset:4096\n\t"
-        "ds_read_b64_tr_b16 %11, %33 offset:6144\n\t"
-        "ds_read_b64_tr_b16 %12, %34 offset:4096\n\t"
-        "ds_read_b64_tr_b16 %13, %34 offset:6144\n\t"
-        "ds_read_b64_tr_b16 %14, %35 offset:4096\n\t"
-        "ds_read_b64_tr_b16 %15, %35 offset:6144\n\t"
-        "ds_read_b64_tr_b16 %16, %32 offset:8192\n\t"
-        "ds_read_b64_tr_b16 %17, %32 offset:10240\n\t"
-        "ds_read_b64_tr_b16 %18, %33 offset:8192\n\t"
-        "ds_read_b64_tr_b16 %19, %33 offset:10240\n\t"
-        "ds_read_b64_tr_b16 %20, %34 offset:8192\n\t"
-        "ds_read_b64_tr_b16 %21, %34 offset:10240\n\t"
-        "ds_read_b64_tr_b16 %22, %35 offset:8192\n\t"
-        "ds_read_b64_tr_b16 %23, %35 offset:10240\n\t"
-        "ds_read_b64_tr_b16 %24, %32 offset:12288\n\t"
-        "ds_read_b64_tr_b16 %25, %32 offset:14336\n\t"
-        "ds_read_b64_tr_b16 %26, %33 offset:12288\n\t"
-        "ds_read_b64_tr_b16 %27, %33 offset:14336\n\t"
-        "ds_read_b64_tr_b16 %28, %34 offset:12288\n\t"
-        "ds_read_b64_tr_b16 %29, %34 offset:14336\n\t"
-        "ds_read_b64_tr_b16 %30, %35 offset:12288\n\t"
-        "ds_read_b64_tr_b16 %31, %35 offset:14336\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(w[4]), "=&v"(w[5]), "=&v"(w[6]), "=&v"(w[7]),
-          "=&v"(w[8]), "=&v"(w[9]), "=&v"(w[10]), "=&v"(w[11]), "=&v"(w[12]), "=&v"(w[13]), "=&v"(w[14]), "=&v"(w[15]),
-          "=&v"(w[16]), "=&v"(w[17]), "=&v"(w[18]), "=&v"(w[19]), "=&v"(w[20]), "=&v"(w[21]), "=&v"(w[22]), "=&v"(w[23]),
-          "=&v"(w[24]), "=&v"(w[25]), "=&v"(w[26]), "=&v"(w[27]), "=&v"(w[28]), "=&v"(w[29]), "=&v"(w[30]), "=&v"(w[31])
-        : "v"(at), "v"(at ^ 64), "v"(at ^ 128), "v"(at ^ 192)
-        : "memory");
-  } else {
-    asm volatile(
-        "ds_read_b64_tr_b16 %0, %16\n\t"
-        "ds_read_b64_tr_b16 %1, %16 offset:1024\n\t"
-        "ds_read_b64_tr_b16 %2, %17\n\t"
-        "ds_read_b64_tr_b16 %3, %17 offset:1024\n\t"
-        "ds_read_b64_tr_b16 %4, %16 offset:2048\n\t"
-        "ds_read_b64_tr_b16 %5, %16 offset:3072\n\t"
-        "ds_read_b64_tr_b16 %6, %17 offset:2048\n\t"
-        "ds_read_b64_tr_b16 %7, %17 offset:3072\n\t"
-        "ds_read_b64_tr_b16 %8, %16 offset:4096\n\t"
-        "ds_read_b64_tr_b16 %9, %16 offset:5120\n\t"
-        "ds_read_b64_tr_b16 %10, %17 offset:4096\n\t"
-        "ds_read_b64_tr_b16 %11, %17 offset:5120\n\t"
-        "ds_read_b64_tr_b16 %12, %16 offset:6144\n\t"
-        "ds_read_b64_tr_b16 %13, %16 offset:7168\n\t"
-        "ds_read_b64_tr_b16 %14, %17 offset:6144\n\t"
-        "ds_read_b64_tr_b16 %15, %17 offset:7168\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(w[4]), "=&v"(w[5]), "=&v"(w[6]), "=&v"(w[7]),
-          "=&v"(w[8]), "=&v"(w[9]), "=&v"(w[10]), "=&v"(w[11]), "=&v"(w[12]), "=&v"(w[13]), "=&v"(w[14]), "=&v"(w[15])
-        : "v"(at), "v"(at ^ 64)
-        : "memory");
-  }
-#pragma unroll
-  for (int s = 0; s < 4; ++s)
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      const u32x2 a = w[(s * (D / 32) + i) * 2], b = w[(s * (D / 32) + i) * 2 + 1];
-      v[s][i] = u32x4{a[0], a[1], b[0], b[1]};
-    }
-}
-
-#define KRN_PHASE()                         \
+#define KRN_BARRIER()                       \
   do {                                      \
-    __builtin_amdgcn_sched_barrier(0);      \
     asm volatile("" ::: "memory");          \
     __builtin_amdgcn_s_barrier();           \
     asm volatile("" ::: "memory");          \
-    __builtin_amdgcn_sched_barrier(0);      \
   } while (0)
 
+// `table` is restrict for what that says about the other memory: without any such word on a transposed LDS read the
+// compiler waits for all loads to LDS before it.
 template <bool BF, int D>
-__global__ __launch_bounds__(512, 2) void cache_prompt(PromptCall c) {
+__device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTile& tile, int column,
+                                            const int* __restrict__ table, uint8_t* lds) {
   constexpr int RB = D * 2, DCH = D / 8, TILE = PROMPT_TILE * RB, LOADS = TILE / 8 / 1024, STEPS = D / 16, BLOCKS = D / 32;
   static_assert(LOADS >= 1, "whole loads a wave");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * PROMPT_RING * TILE];
-  const int column = (int)(blockIdx.x % c.kv_heads), slot = c.slots - 1 - (int)(blockIdx.x / c.kv_heads);
-  PromptTile tile;
-  if (!find_tile(c, slot, tile)) return;
   const int t = threadIdx.x, lane = t & 63, half = lane >> 5, r32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int length = __builtin_amdgcn_readfirstlane(sequence_length(c.s, tile.seq));
@@ -193,13 +111,12 @@ __global__ __launch_bounds__(512, 2) void cache_prompt(PromptCall c) {
     koff[i] = (uint32_t)(key * RB + k_slot<D>(in_tile, s) * 16);
     voff[i] = (uint32_t)(key * RB + v_slot<D>(in_tile, s) * 16);
   }
-  const __attribute__((address_space(4))) int* table =
-      (const __attribute__((address_space(4))) int*)(uintptr_t)(c.s.table + (int64_t)tile.seq * c.s.width);
   const int shift = c.cache.page_shift;
-  // the page of this wave's group in tile u, or -1
+  // the page of this wave's group in tile u, or -1; without a branch, which would draw the work around it into its blocks
   const auto page_of = [&](int u) {
     const int at = ((first + u) * PROMPT_TILE + group * 16) >> shift;
-    return u < n && at < c.s.width ? table[at] : -1;
+    const int number = ((const __attribute__((address_space(4))) int*)(uintptr_t)table)[max(0, min(at, c.s.width - 1))];
+    return u < n && at < c.s.width ? number : -1;
   };
   const auto load = [&](const void* data, int number, int u, int ring, const uint32_t(&off)[LOADS]) {
     const int key0 = (first + u) * PROMPT_TILE + group * 16;
@@ -214,86 +131,124 @@ __global__ __launch_bounds__(512, 2) void cache_prompt(PromptCall c) {
   const auto ring_of = [](int u) { return (u & (PROMPT_RING - 1)) * TILE; };
 
   // fragments: K's as A operands (lane = key, 8 columns of step s), V^T's (lane = column, keys as the lane's P has them)
-  const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-  const uint32_t kat = lds_at + r32 * RB + k_slot<D>(r32, half) * 16;
+  const uint32_t kat = r32 * RB + k_slot<D>(r32, half) * 16;
   const int a16 = lane & 15, tr_key = (lane >> 5) * 4 + (a16 >> 2), tr_col = ((lane >> 4) & 1) * 16 + 4 * (a16 & 3);
-  const uint32_t vat = lds_at + V_RING + tr_key * RB + v_slot<D>(tr_key, tr_col >> 3) * 16 + (tr_col & 7) * 2;
-  u32x4 kf[2][STEPS];
-  const auto read_keys = [&](int ring) {
-    const uint32_t at = kat + ring;
+  const uint32_t vat = V_RING + tr_key * RB + v_slot<D>(tr_key, tr_col >> 3) * 16 + (tr_col & 7) * 2;
+  constexpr int K_AHEAD = 3, V_AHEAD = 2;  // steps whose fragments are held
+  u32x4 kf[K_AHEAD][2], vf[V_AHEAD][BLOCKS];
+  const auto read_keys = [&](uint32_t at, int s) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s)
-        kf[h][s] = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)((at ^ (s << 5)) + h * 32 * RB);
+    for (int h = 0; h < 2; ++h) kf[s % K_AHEAD][h] = *reinterpret_cast<const u32x4*>(lds + ((at ^ (s << 5)) + h * 32 * RB));
   };
-  u32x4 vf[4][BLOCKS];
+  const auto read_values = [&](uint32_t at, int s, int i) {
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) v4s*)(lds + ((at ^ (i << 6)) + (s * 16 + part * 8) * RB))));
+      vf[s % V_AHEAD][i][part * 2] = w[0], vf[s % V_AHEAD][i][part * 2 + 1] = w[1];
+    }
+  };
 
   f32x16 acc[BLOCKS];
 #pragma unroll
   for (int i = 0; i < BLOCKS; ++i) acc[i] = f32x16{};
-  float m = -INFINITY, base = 0.0f, total = 0.0f;  // base: m, or 0 while no key has been seen
-  f32x16 s0, s1;  // scores of both halves
+  // a score's exponent is s scale - base; exponents above `margin` move the base: the first one, then those above 8
+  float base = 0.0f, margin = -INFINITY, total = 0.0f;
   u32x4 pf[4];
-  const auto scores = [&]() {
-    s0 = f32x16{}, s1 = f32x16{};
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      Half<BF>::mma(s0, kf[0][s], qf[s]);
-      Half<BF>::mma(s1, kf[1][s], qf[s]);
+
+  // The weights of a tile from its exponents, 2^x packed as P^T, in 34 pieces of work, each on two of a lane's 32: piece 2 x
+  // raises 2 to pair x, 2 x + 1 adds up and packs pair x - 1
+  constexpr int PIECES = 34;
+  const auto piece = [&](f32x16(&s)[2], int at) {
+    const int pair = at / 2 - at % 2;
+    if (pair < 0 || pair > 15) return;
+    f32x16& v = s[pair / 8];
+    const int e = pair % 8 * 2;
+    if (at % 2 == 0) {
+      v[e] = __builtin_amdgcn_exp2f(v[e]), v[e + 1] = __builtin_amdgcn_exp2f(v[e + 1]);
+    } else {
+      total += v[e] + v[e + 1];
+      pf[pair / 4][pair % 4] = Half<BF>::pack(v[e], v[e + 1]);
     }
   };
-  // weights of one half: p = 2^(s scale - base), packed as two steps of P^T
-  const auto weights = [&](const f32x16& s, int h) {
-    float sum = 0.0f;
-#pragma unroll
-    for (int step = 0; step < 2; ++step)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[step * 8 + 2 * e], c.scale, -base));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[step * 8 + 2 * e + 1], c.scale, -base));
-        sum += p0 + p1;
-        pf[h * 2 + step][e] = Half<BF>::pack(p0, p1);
-      }
-    total += sum;
+  // exponents of a pair of scores, and their largest (scaled ones: the compiler quiets a product's scores first)
+  const auto scaled = [&](f32x16& v, int e, float& top) {
+    v[e] = __builtin_fmaf(v[e], c.scale, -base), v[e + 1] = __builtin_fmaf(v[e + 1], c.scale, -base);
+    top = fmaxf(fmaxf(top, v[e]), v[e + 1]);
   };
-  // the maximum and the weights of tile u
-  const auto begin = [&](int u) {
+  // Masks the exponents of tile u, whose largest is `top` before that, and settles the base: it moves only when a weight would
+  // exceed 2^8, and then exponents, acc and total with it.
+  const auto settle = [&](f32x16(&s)[2], float top, int u) {
     const int key0 = (first + u) * PROMPT_TILE;
     if (key0 < all_low || key0 + PROMPT_TILE > all_limit) {
+      top = -INFINITY;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int key = key0 + half * 4 + (r >> 2) * 8 + (r & 3);
-        s0[r] = key >= limit || key < low ? -INFINITY : s0[r];
-        s1[r] = key + 32 >= limit || key + 32 < low ? -INFINITY : s1[r];
+        s[0][r] = key >= limit || key < low ? -INFINITY : s[0][r];
+        s[1][r] = key + 32 >= limit || key + 32 < low ? -INFINITY : s[1][r];
+        top = fmaxf(top, fmaxf(s[0][r], s[1][r]));
       }
     }
-    float top = s0[0];
-#pragma unroll
-    for (int r = 1; r < 16; ++r) top = fmaxf(top, s0[r]);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) top = fmaxf(top, s1[r]);
-    top *= c.scale;
-    // the base moves only when a weight would exceed 2^8: then acc and total are rescaled
-    if (__builtin_amdgcn_ballot_w64(top > m + 8.0f) != 0) {
-      const float next = fmaxf(m, pair_max(top)), to_base = next == -INFINITY ? 0.0f : next;
-      const float corr = __builtin_amdgcn_exp2f(m - to_base);
+    if (__builtin_amdgcn_ballot_w64(top > margin) != 0) {
+      top = pair_max(top);
+      const bool moves = top > margin, began = margin == 8.0f;
+      const float by = moves ? top : 0.0f, corr = moves && began ? __builtin_amdgcn_exp2f(-by) : 1.0f;
       total *= corr;
 #pragma unroll
       for (int i = 0; i < BLOCKS; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][r] *= corr;
-      m = next, base = to_base;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[0][r] -= by, s[1][r] -= by;
+      base += by;
+      margin = moves ? 8.0f : margin;
     }
-    weights(s0, 0);
-    weights(s1, 1);
+  };
+  // Tile u, whose exponents `s` are settled: the scores `next` of tile u + 1 beside most weights of u, then O += P V beside the
+  // others and the exponents of u + 1. One MFMA and a little of the other work at a time, in this order.
+  const auto step = [&](f32x16(&s)[2], f32x16(&next)[2], int u, int& next_k, int& next_v) {
+    const uint32_t k_at = kat + ring_of(u + 1), k_then = kat + ring_of(u + 2), v_at = vat + ring_of(u);
+    constexpr int FIRST = 24, SCORES = 2 * STEPS, PRODUCTS = 4 * BLOCKS;
+    next[0] = f32x16{}, next[1] = f32x16{};
+#pragma unroll
+    for (int i = 0; i < SCORES; ++i) {
+      if (i % 2 == 0 && i / 2 + 2 < STEPS) read_keys(k_at, i / 2 + 2);
+      if (i >= SCORES - BLOCKS) read_values(v_at, 0, i - (SCORES - BLOCKS));
+      Half<BF>::mma(next[i % 2], kf[i / 2 % K_AHEAD][i % 2], qf[i / 2]);
+#pragma unroll
+      for (int x = i * FIRST / SCORES; x < (i + 1) * FIRST / SCORES; ++x) piece(s, x);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * LOADS) : "memory");  // this wave's part of K of u + 2 and V of u + 1
+    KRN_BARRIER();
+    __builtin_amdgcn_sched_barrier(0);
+    load(c.cache.values, next_v, u + 3, V_RING + ring_of(u + 3), voff);
+    load(c.cache.keys, next_k, u + 5, ring_of(u + 1), koff);
+    float top[2] = {-INFINITY, -INFINITY};
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < PRODUCTS; ++i) {
+      if (i / BLOCKS < 3) read_values(v_at, i / BLOCKS + 1, i % BLOCKS);
+      if (i >= PRODUCTS - 4 && i % 2 == 0) read_keys(k_then, (i - (PRODUCTS - 4)) / 2);
+      Half<BF>::mma(acc[i % BLOCKS], vf[i / BLOCKS % V_AHEAD][i % BLOCKS], pf[i / BLOCKS]);
+      constexpr int LAST = 3 * BLOCKS;  // products before those of the last weights
+      if (i < LAST)
+#pragma unroll
+        for (int x = FIRST + i * (PIECES - FIRST) / LAST; x < FIRST + (i + 1) * (PIECES - FIRST) / LAST; ++x) piece(s, x);
+#pragma unroll
+      for (int x = i * 16 / PRODUCTS; x < (i + 1) * 16 / PRODUCTS; ++x) scaled(next[x / 8], x % 8 * 2, top[x / 8]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    asm volatile("" : "+v"(top[0]), "+v"(top[1]), "+v"(total));  // here, not in the branches that follow
+    next_v = page_of(u + 4), next_k = page_of(u + 6);
+    settle(next, fmaxf(top[0], top[1]), u + 1);
   };
 
-  // page numbers one load ahead
-  int k_page[PROMPT_RING], next_k, next_v;
+  // tiles on their way in the order that the loop keeps: V of u + 3, then K of u + 5
+  int k_page[6];
 #pragma unroll
-  for (int u = 0; u < PROMPT_RING; ++u) k_page[u] = page_of(u);
-  next_k = page_of(PROMPT_RING), next_v = k_page[3];
+  for (int u = 0; u < 6; ++u) k_page[u] = page_of(u);
   load(c.cache.keys, k_page[0], 0, ring_of(0), koff);
   load(c.cache.keys, k_page[1], 1, ring_of(1), koff);
   load(c.cache.values, k_page[0], 0, V_RING + ring_of(0), voff);
@@ -304,38 +259,33 @@ __global__ __launch_bounds__(512, 2) void cache_prompt(PromptCall c) {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * LOADS) : "memory");  // the first two K tiles and the first V tile
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) asm volatile("" : "+v"(qf[s]));  // older loads: no wait for them in the loop
-  KRN_PHASE();
-  read_keys(ring_of(0));
-  scores();
-  begin(0);
-  read_keys(ring_of(1));
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  KRN_PHASE();  // everyone has read the first tile: its place may be loaded
-  if (wave >= 4) KRN_PHASE();
-  for (int u = 0; u < n; ++u) {
-    load(c.cache.keys, next_k, u + 4, ring_of(u), koff);
-    load(c.cache.values, next_v, u + 3, V_RING + ring_of(u + 3), voff);
-    __builtin_amdgcn_s_setprio(1);
-    scores();
-    asm volatile("" : "+v"(s0), "+v"(s1));  // here, not where they are used
-    __builtin_amdgcn_s_setprio(0);
-    KRN_PHASE();
-    value_tile<D>(vat + ring_of(u), vf);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * LOADS) : "memory");  // K of u + 2 and V of u + 1
-    KRN_PHASE();
-    __builtin_amdgcn_s_setprio(1);
+  KRN_BARRIER();
+  f32x16 sa[2], sb[2];
+  sa[0] = f32x16{}, sa[1] = f32x16{};
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int i = 0; i < BLOCKS; ++i) Half<BF>::mma(acc[i], vf[s][i], pf[s]);
-    __builtin_amdgcn_s_setprio(0);
-    KRN_PHASE();
-    next_v = next_k, next_k = page_of(u + 5);
-    read_keys(ring_of(u + 2));
-    if (u + 1 < n) begin(u + 1);
-    KRN_PHASE();
+  for (int s = 0; s < STEPS; ++s) {
+    read_keys(kat, s);
+    Half<BF>::mma(sa[0], kf[s % K_AHEAD][0], qf[s]);
+    Half<BF>::mma(sa[1], kf[s % K_AHEAD][1], qf[s]);
   }
-  if (wave < 4) KRN_PHASE();
+  {
+    float top = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < 16; ++x) scaled(sa[x / 8], x % 8 * 2, top);
+    settle(sa, top, 0);
+  }
+  read_keys(kat + ring_of(1), 0);
+  read_keys(kat + ring_of(1), 1);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  KRN_BARRIER();  // everyone has read the first tile: its place may be loaded
+  load(c.cache.keys, k_page[4], 4, ring_of(0), koff);
+  int next_k = k_page[5], next_v = k_page[3];
+  for (int u = 0;;) {
+    step(sa, sb, u, next_k, next_v);
+    if (++u >= n) break;
+    step(sb, sa, u, next_k, next_v);
+    if (++u >= n) break;
+  }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may reach LDS after the workgroup
 
   {
@@ -365,7 +315,16 @@ __global__ __launch_bounds__(512, 2) void cache_prompt(PromptCall c) {
       if (real) *reinterpret_cast<u32x4*>(c.o + place + i * 32 + (2 * gp + half) * 8) = piece;
     }
 }
-#undef KRN_PHASE
+#undef KRN_BARRIER
+
+template <bool BF, int D>
+__global__ __launch_bounds__(512, 2) void cache_prompt(PromptCall c) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * PROMPT_RING * PROMPT_TILE * D * 2];
+  const int column = (int)(blockIdx.x % c.kv_heads), slot = c.slots - 1 - (int)(blockIdx.x / c.kv_heads);
+  PromptTile tile;
+  if (!find_tile(c, slot, tile)) return;
+  prompt_tile<BF, D>(c, tile, column, c.s.table + (int64_t)tile.seq * c.s.width, lds);
+}
 
 }  // namespace krn
 
