@@ -18,8 +18,10 @@ static TokenPlan plan_of(int64_t tokens, int64_t heads, int64_t kv_heads, int64_
 
 extern "C" int64_t krn_cache_attention_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t d, int64_t page,
                                                  int packed, int64_t sequences, int64_t width) {
-  if (packed || tokens <= 0 || sequences <= 0 || heads <= 0 || kv_heads <= 0 || width <= 0) return 0;
-  if (tokens / sequences * (heads / kv_heads) > TOKEN_ROWS) return 0;
+  if (tokens <= 0 || sequences <= 0 || kv_heads <= 0 || heads < kv_heads || width <= 0 || page <= 0) return 0;
+  const int64_t group = heads / kv_heads, step = packed ? 0 : tokens / sequences;
+  if (packed || step * group > TOKEN_ROWS)
+    return prompt_plan(tokens, step, group, kv_heads, d, page, sequences, width, INT64_MAX).bytes;
   return plan_of(tokens, heads, kv_heads, d, page, sequences, width, INT64_MAX).bytes;
 }
 
@@ -74,14 +76,17 @@ extern "C" int krn_cache_attention(int kind, const void* q, const void* keys, co
     c.window = span, c.scale = by;
     launch_cache_tokens(kind == BF16, (int)d, c, p, workspace, (hipStream_t)stream);
   } else {
-    const int64_t slots = prompt_slots(tokens, starts ? 0 : step, group, sequences);
-    if (slots * kv_heads >= (int64_t)1 << 23) {
+    const PromptPlan p = prompt_plan(tokens, starts ? 0 : step, group, kv_heads, d, page, sequences, width,
+                                     workspace ? workspace_bytes : 0);
+    if (p.workgroups * kv_heads >= (int64_t)1 << 23) {
       krn_set_error("cache_attention: %lld tokens of %lld sequences and %lld heads", (long long)tokens, (long long)sequences,
                     (long long)heads);
       return -1;
     }
-    const PromptCall c{(const uint16_t*)q, (uint16_t*)o, cache, s, (int)heads, (int)kv_heads, group, span, (int)slots, by};
-    launch_cache_prompt(kind == BF16, (int)d, c, (hipStream_t)stream);
+    PromptCall c{};
+    c.q = (const uint16_t*)q, c.o = (uint16_t*)o, c.cache = cache, c.s = s, c.heads = (int)heads, c.kv_heads = (int)kv_heads;
+    c.group = group, c.window = span, c.scale = by;
+    launch_cache_prompt(kind == BF16, (int)d, c, p, workspace, (hipStream_t)stream);
   }
   const hipError_t err = hipGetLastError();
   if (err == hipSuccess) return 0;

@@ -37,6 +37,21 @@ __device__ __forceinline__ int first_key(int position, int window) {
   return window ? (int)max((int64_t)0, (int64_t)position + 1 - window) : 0;
 }
 
+// The sum over lanes up to this one: rows of sixteen by shifts, then the rows' ends
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t from_lane(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x += from_lane<0x111, 0xf>(x);
+  x += from_lane<0x112, 0xf>(x);
+  x += from_lane<0x114, 0xf>(x);
+  x += from_lane<0x118, 0xf>(x);
+  x += from_lane<0x142, 0xa>(x);  // lane 15 to the second row, lane 47 to the fourth
+  x += from_lane<0x143, 0xc>(x);  // lane 31 to the upper half
+  return x;
+}
+
 // Attention of new tokens, a few of every sequence (cache_token.hip)
 constexpr int TOKEN_WAVES = 4;
 constexpr int TOKEN_ROWS = 64;     // rows of a key head, at most; more are a prompt's
@@ -70,17 +85,28 @@ void launch_cache_tokens(bool bf, int d, TokenCall c, const TokenPlan& p, void* 
 // Attention of packed prompts (cache_prompt.hip)
 constexpr int PROMPT_ROWS = 256;  // of a workgroup: tokens times query heads of a key head
 
+constexpr int PROMPT_CHUNK = 16;  // tiles of 64 keys of a part, at least
+constexpr int PROMPT_CUS = 256;   // workgroups that run at once
+
 struct PromptCall {
   const uint16_t* q;
   uint16_t* o;
   CacheView cache;
   SequencesView s;
-  int heads, kv_heads, group, window, slots;  // group: query heads of a key head
-  float scale;                                // of the scores, times log2(e)
+  int heads, kv_heads, group, window;  // group: query heads of a key head
+  float scale;                         // of the scores, times log2(e)
+  int slots;        // workgroups of a key head without parts
+  uint32_t shares;  // workgroups of a key head with parts, or 0
+  int4* header;     // the number of tiles of rows in several parts, then of each (sequence, first row, first workgroup, parts)
+  float* planes;    // of a workgroup: 256 rows of sums, then their bases and sums of weights
 };
-// Workgroups of a key head: without starts those of `step` tokens a sequence, else enough for any lengths (step 0)
-int64_t prompt_slots(int64_t tokens, int64_t step, int64_t group, int64_t sequences);
-void launch_cache_prompt(bool bf, int d, const PromptCall& c, hipStream_t stream);
+// slots: tiles of rows of a key head, without starts those of `step` tokens a sequence, else enough for any lengths (step 0)
+struct PromptPlan {
+  int64_t slots, shares, workgroups, joins, header_bytes, bytes;
+};
+PromptPlan prompt_plan(int64_t tokens, int64_t step, int64_t group, int64_t kv_heads, int64_t d, int64_t page, int64_t sequences,
+                       int64_t width, int64_t bytes);
+void launch_cache_prompt(bool bf, int d, PromptCall c, const PromptPlan& p, void* workspace, hipStream_t stream);
 
 }  // namespace krn
 

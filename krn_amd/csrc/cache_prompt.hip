@@ -60,6 +60,78 @@ __device__ __forceinline__ bool find_tile(const PromptCall& c, int slot, PromptT
   return at >= 0 && (int64_t)at * PROMPT_ROWS < (int64_t)tile.range.count * c.group;
 }
 
+// The key tiles that 256 rows from row0 on see: from the first row's window to the last row's position
+struct KeyTiles {
+  int first, count;
+};
+__device__ __forceinline__ KeyTiles tiles_seen(const PromptCall& c, const TokenRange& range, int length, int row0) {
+  const int before = length - range.count, last = min((row0 + PROMPT_ROWS - 1) / c.group, range.count - 1);
+  const int end = min(before + last + 1, held_keys(c.s, length, c.cache.page_shift));
+  const int first = first_key(before + row0 / c.group, c.window) / PROMPT_TILE;
+  return {first, max(0, (max(end, 0) + PROMPT_TILE - 1) / PROMPT_TILE - first)};
+}
+
+// The key tiles of few tiles of rows are shared out: workgroup w of a column does part `part` of `parts` of some rows, the
+// `order`-th of those in several parts. A part has at most chunk tiles, chunk such that the parts fill the chip once: with S shares of a
+// column and R tiles of rows, T / (S - R). Every wave counts for itself, a lane for ceil(n / 64) sequences in a row.
+struct PromptPart {
+  int part, parts, order;
+};
+__device__ __forceinline__ bool find_part(const PromptCall& c, int w, bool writes, PromptTile& tile, PromptPart& share) {
+  const int lane = threadIdx.x & 63, per = (c.s.n + 63) / 64, from = lane * per, to = min(from + per, c.s.n);
+  const auto weight_of = [&](const TokenRange& r, int length, int k) {  // capped: the sum of all stays below 2^32
+    return (uint32_t)min(tiles_seen(c, r, length, k * PROMPT_ROWS).count, 1 << 23);
+  };
+  const auto rows_of = [&](const TokenRange& r) { return (r.count * c.group + PROMPT_ROWS - 1) / PROMPT_ROWS; };
+  uint32_t tiles = 0, items = 0;
+  for (int i = from; i < to; ++i) {
+    const TokenRange range = token_range(c.s, i);
+    const int length = sequence_length(c.s, i), rows = rows_of(range);
+    items += rows;
+    for (int k = 0; k < rows; ++k) tiles += weight_of(range, length, k);
+  }
+  tiles = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(tiles), 63);
+  items = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(items), 63);
+  const uint32_t spare = items < c.shares ? c.shares - items : 1;
+  const uint32_t chunk = items < c.shares ? max((uint32_t)PROMPT_CHUNK, (tiles + spare - 1) / spare) : 0x7fffffff;
+  // parts in the low half, rows in several of them in the high one
+  uint32_t count = 0;
+  for (int i = from; i < to; ++i) {
+    const TokenRange range = token_range(c.s, i);
+    const int length = sequence_length(c.s, i), rows = rows_of(range);
+    for (int k = 0; k < rows; ++k) {
+      const uint32_t parts = max(1u, (weight_of(range, length, k) + chunk - 1) / chunk);
+      count += parts + (parts > 1 ? 0x10000u : 0u);
+    }
+  }
+  const uint32_t upto = wave_scan(count), all = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+  if (writes && w == 0 && threadIdx.x == 0) c.header[0] = {items < c.shares ? (int)(all >> 16) : 0, 0, 0, 0};
+  uint32_t before = upto - count;
+  const uint64_t owner = __builtin_amdgcn_ballot_w64((int)(before & 0xffff) <= w && w < (int)(upto & 0xffff));
+  if (owner == 0) return false;
+  int seq = 0, at = 0, parts = 0;
+  for (int i = from; i < to && parts == 0; ++i) {  // in the owner's lane: the rows
+    const TokenRange range = token_range(c.s, i);
+    const int length = sequence_length(c.s, i), rows = rows_of(range);
+    for (int k = 0; k < rows; ++k) {
+      const int p = (int)max(1u, (weight_of(range, length, k) + chunk - 1) / chunk);
+      if (w < (int)(before & 0xffff) + p) {
+        seq = i, at = k, parts = p;
+        break;
+      }
+      before += p + (p > 1 ? 0x10000u : 0u);
+    }
+  }
+  const int of = __builtin_ctzll(owner);
+  tile.seq = __builtin_amdgcn_readlane(seq, of), tile.row0 = __builtin_amdgcn_readlane(at, of) * PROMPT_ROWS;
+  tile.range = token_range(c.s, tile.seq);
+  tile.range.first = __builtin_amdgcn_readfirstlane(tile.range.first);
+  tile.range.count = __builtin_amdgcn_readfirstlane(tile.range.count);
+  before = (uint32_t)__builtin_amdgcn_readlane((int)before, of);
+  share.parts = __builtin_amdgcn_readlane(parts, of), share.part = w - (int)(before & 0xffff), share.order = (int)(before >> 16);
+  return share.parts > 0;  // always, where starts do not decrease
+}
+
 #define KRN_BARRIER()                       \
   do {                                      \
     asm volatile("" ::: "memory");          \
@@ -70,8 +142,8 @@ __device__ __forceinline__ bool find_tile(const PromptCall& c, int slot, PromptT
 // `table` is restrict for what that says about the other memory: without any such word on a transposed LDS read the
 // compiler waits for all loads to LDS before it.
 template <bool BF, int D>
-__device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTile& tile, int column,
-                                            const int* __restrict__ table, uint8_t* lds) {
+__device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTile& tile, int column, int part, int parts,
+                                            float* plane, const int* __restrict__ table, uint8_t* lds) {
   constexpr int RB = D * 2, DCH = D / 8, TILE = PROMPT_TILE * RB, LOADS = TILE / 8 / 1024, STEPS = D / 16, BLOCKS = D / 32;
   static_assert(LOADS >= 1, "whole loads a wave");
   const int t = threadIdx.x, lane = t & 63, half = lane >> 5, r32 = lane & 31;
@@ -85,12 +157,12 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
   const bool real = j < tile.range.count;
   const int limit = min(before + min(j, tile.range.count - 1) + 1, end), low = first_key(before + min(j, tile.range.count - 1), c.window);
   const int all_limit = __builtin_amdgcn_readfirstlane(limit), all_low = __builtin_amdgcn_readlane(low, 31);
-  const int last_token = __builtin_amdgcn_readfirstlane(min((tile.row0 + PROMPT_ROWS - 1) / c.group, tile.range.count - 1));
-  const int key_end = min(before + last_token + 1, end);
-  const int first = __builtin_amdgcn_readfirstlane(first_key(before + tile.row0 / c.group, c.window) / PROMPT_TILE);
-  const int n = __builtin_amdgcn_readfirstlane((key_end + PROMPT_TILE - 1) / PROMPT_TILE) - first;
+  const KeyTiles seen = tiles_seen(c, tile.range, length, tile.row0);
+  const int even = __builtin_amdgcn_readfirstlane(seen.count / parts), over = seen.count - even * parts;
+  const int first = __builtin_amdgcn_readfirstlane(seen.first + even * part + min(part, over));
+  const int n = __builtin_amdgcn_readfirstlane(even + (part < over ? 1 : 0));
   const int64_t place = ((int64_t)(tile.range.first + j) * c.heads + column * c.group + (row - j * c.group)) * D;
-  if (n <= 0 || key_end <= 0) {  // no row sees a key
+  if (n <= 0) {  // no row sees a key
     if (real)
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) *reinterpret_cast<u32x4*>(c.o + place + s * 16 + half * 8) = u32x4{};
@@ -292,6 +364,20 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(total), __float_as_uint(total), false, false);
     total = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
   }
+  if (parts > 1) {  // unnormalised rows, then their bases and sums
+    float* at = plane + (wave * 32 + r32) * D + half * 4;
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i)
+#pragma unroll
+      for (int gq = 0; gq < 4; ++gq)
+        *reinterpret_cast<f32x4*>(at + i * 32 + gq * 8) =
+            f32x4{acc[i][gq * 4], acc[i][gq * 4 + 1], acc[i][gq * 4 + 2], acc[i][gq * 4 + 3]};
+    if (half == 0) {
+      plane[PROMPT_ROWS * D + (wave * 32 + r32) * 2] = margin == 8.0f ? base : -INFINITY;
+      plane[PROMPT_ROWS * D + (wave * 32 + r32) * 2 + 1] = total;
+    }
+    return;
+  }
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // no key: zeros
   // lane (r32, half) has columns i * 32 + gq * 8 + half * 4 to + 3; its partner's four complete 16 bytes
 #pragma unroll
@@ -320,25 +406,79 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
 template <bool BF, int D>
 __global__ __launch_bounds__(512, 2) void cache_prompt(PromptCall c) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * PROMPT_RING * PROMPT_TILE * D * 2];
-  const int column = (int)(blockIdx.x % c.kv_heads), slot = c.slots - 1 - (int)(blockIdx.x / c.kv_heads);
+  const int w = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / c.kv_heads)), column = (int)blockIdx.x - w * c.kv_heads;
   PromptTile tile;
-  if (!find_tile(c, slot, tile)) return;
-  prompt_tile<BF, D>(c, tile, column, c.s.table + (int64_t)tile.seq * c.s.width, lds);
+  PromptPart share{0, 1, 0};
+  if (c.shares) {
+    if (!find_part(c, w, column == 0, tile, share)) return;
+    if (share.parts > 1 && share.part == 0 && column == 0 && threadIdx.x == 0)
+      c.header[1 + share.order] = {tile.seq, tile.row0, w, share.parts};
+  } else if (!find_tile(c, c.slots - 1 - w, tile)) {  // late rows, the long ones, first
+    return;
+  }
+  float* plane = c.planes + ((int64_t)w * c.kv_heads + column) * (PROMPT_ROWS * (D + 2));
+  prompt_tile<BF, D>(c, tile, column, share.part, share.parts, plane, c.s.table + (int64_t)tile.seq * c.s.width, lds);
+}
+
+// Rows in several parts: four columns of a row a thread, the parts one after the other
+template <bool BF, int D>
+__global__ __launch_bounds__(256) void cache_prompt_join(PromptCall c) {
+  constexpr int ROWS = 256 / (D / 4), BLOCKS = PROMPT_ROWS / ROWS;  // of a workgroup, of a tile of rows
+  const int column = (int)(blockIdx.x % c.kv_heads), rest = (int)(blockIdx.x / c.kv_heads), order = rest / BLOCKS;
+  if (order >= c.header[0].x) return;
+  const int4 head = c.header[1 + order];
+  const TokenRange range = token_range(c.s, head.x);
+  const int r = rest % BLOCKS * ROWS + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+  const int row = head.y + r, j = row / c.group;
+  if (j >= range.count) return;
+  const int64_t stride = (int64_t)c.kv_heads * (PROMPT_ROWS * (D + 2));
+  const float* plane = c.planes + head.z * stride + (int64_t)column * (PROMPT_ROWS * (D + 2));
+  float top = -INFINITY;
+  for (int p = 0; p < head.w; ++p) top = fmaxf(top, plane[p * stride + PROMPT_ROWS * D + r * 2]);
+  const float to_base = top == -INFINITY ? 0.0f : top;
+  float all = 0.0f;
+  f32x4 o = f32x4{};
+#pragma unroll 4
+  for (int p = 0; p < head.w; ++p) {
+    const float* at = plane + p * stride;
+    const float f = __builtin_amdgcn_exp2f(at[PROMPT_ROWS * D + r * 2] - to_base);
+    all += f * at[PROMPT_ROWS * D + r * 2 + 1];
+    o += f * *reinterpret_cast<const f32x4*>(at + r * D + d);
+  }
+  const float inv = all == 0.0f ? 0.0f : 1.0f / all;  // no key: zeros
+  const u32x2 y = {Half<BF>::pack(o[0] * inv, o[1] * inv), Half<BF>::pack(o[2] * inv, o[3] * inv)};
+  *reinterpret_cast<u32x2*>(c.o + ((int64_t)(range.first + j) * c.heads + column * c.group + (row - j * c.group)) * D + d) = y;
 }
 
 }  // namespace krn
 
 using namespace krn;
 
-int64_t krn::prompt_slots(int64_t tokens, int64_t step, int64_t group, int64_t sequences) {
-  if (step > 0) return sequences * ((step * group + PROMPT_ROWS - 1) / PROMPT_ROWS);
-  return tokens * group / PROMPT_ROWS + sequences;
+PromptPlan krn::prompt_plan(int64_t tokens, int64_t step, int64_t group, int64_t kv_heads, int64_t d, int64_t page,
+                            int64_t sequences, int64_t width, int64_t bytes) {
+  PromptPlan p{};
+  p.slots = p.workgroups = step > 0 ? sequences * ((step * group + PROMPT_ROWS - 1) / PROMPT_ROWS)
+                                    : tokens * group / PROMPT_ROWS + sequences;
+  const int64_t shares = PROMPT_CUS / kv_heads;
+  if (width * page / PROMPT_TILE <= PROMPT_CHUNK || p.slots >= shares) return p;
+  // parts: as many as shares where there are fewer rows than that, else one each; at least two of every row that has several
+  const int64_t header = (shares / 2 + 1) * 16, need = header + shares * kv_heads * PROMPT_ROWS * (d + 2) * 4;
+  if (need > bytes) return p;
+  p.shares = p.workgroups = shares, p.joins = shares / 2, p.header_bytes = header, p.bytes = need;
+  return p;
 }
 
-void krn::launch_cache_prompt(bool bf, int d, const PromptCall& c, hipStream_t stream) {
-  const dim3 grid((unsigned)(c.slots * c.kv_heads)), block(512);
-  if (bf && d == 128) hipLaunchKernelGGL((cache_prompt<true, 128>), grid, block, 0, stream, c);
-  else if (bf) hipLaunchKernelGGL((cache_prompt<true, 64>), grid, block, 0, stream, c);
-  else if (d == 128) hipLaunchKernelGGL((cache_prompt<false, 128>), grid, block, 0, stream, c);
-  else hipLaunchKernelGGL((cache_prompt<false, 64>), grid, block, 0, stream, c);
+template <bool BF, int D>
+static void launch(const PromptCall& c, const PromptPlan& p, hipStream_t stream) {
+  hipLaunchKernelGGL((cache_prompt<BF, D>), dim3((unsigned)(p.workgroups * c.kv_heads)), dim3(512), 0, stream, c);
+  if (p.shares)
+    hipLaunchKernelGGL((cache_prompt_join<BF, D>), dim3((unsigned)(p.joins * (PROMPT_ROWS * (D / 4) / 256) * c.kv_heads)),
+                       dim3(256), 0, stream, c);
+}
+
+void krn::launch_cache_prompt(bool bf, int d, PromptCall c, const PromptPlan& p, void* workspace, hipStream_t stream) {
+  c.slots = (int)p.slots, c.shares = (uint32_t)p.shares;
+  c.header = (int4*)workspace, c.planes = (float*)((char*)workspace + p.header_bytes);
+  if (bf) d == 128 ? launch<true, 128>(c, p, stream) : launch<true, 64>(c, p, stream);
+  else d == 128 ? launch<false, 128>(c, p, stream) : launch<false, 64>(c, p, stream);
 }

@@ -118,21 +118,6 @@ struct Share {
   int seq, part, parts, order;
 };
 
-// the sum over lanes up to this one: rows of sixteen by shifts, then the rows' ends
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t from_lane(uint32_t x) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
-  x += from_lane<0x111, 0xf>(x);
-  x += from_lane<0x112, 0xf>(x);
-  x += from_lane<0x114, 0xf>(x);
-  x += from_lane<0x118, 0xf>(x);
-  x += from_lane<0x142, 0xa>(x);  // lane 15 to the second row, lane 47 to the fourth
-  x += from_lane<0x143, 0xc>(x);  // lane 31 to the upper half
-  return x;
-}
-
 // Every wave counts for itself, a lane for ceil(n / 64) sequences in a row, so that no barrier is needed.
 __device__ __forceinline__ bool find_share(const TokenCall& c, int w, bool writes, Share& share) {
   if (!c.split) {

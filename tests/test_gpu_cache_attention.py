@@ -19,6 +19,9 @@ PACKED = [
     ([17] * 9, list(range(9)), 3, 3, 128, 16, 0), ([70, 9], [500, 1000], 5, 1, 64, 128, 0), ([257], [0], 2, 2, 128, 256, 0),
     ([90], [40], 4, 2, 128, 16, 1), ([90], [40], 4, 2, 64, 16, 33), ([200, 31], [400, 0], 8, 2, 128, 32, 100),
     ([1] * 70, [11] * 70, 16, 1, 64, 16, 0), ([40], [0], 48, 1, 64, 16, 0), ([513], [70], 1, 1, 64, 16, 64),
+    # few rows, many keys: the keys of a tile of rows in several parts
+    ([40], [3000], 4, 1, 128, 16, 0), ([150, 5], [2500, 4000], 8, 2, 64, 32, 0), ([60, 0, 90], [5000, 9, 1], 4, 2, 128, 64, 3000),
+    ([3, 200], [7000, 1500], 3, 3, 64, 128, 0), ([1] * 5, [2000, 1, 1500, 40, 3000], 8, 1, 128, 16, 0),
 ]  # fmt: skip
 # lengths, new tokens each, heads, kv_heads, d, page, window
 TOKENS = [
@@ -27,7 +30,7 @@ TOKENS = [
     ([5000], 1, 16, 1, 128, 64, 0), ([300, 40], 1, 17, 1, 64, 16, 0), ([200, 3], 1, 40, 1, 128, 16, 0),
     ([700, 9, 31], 3, 4, 2, 128, 16, 0), ([64, 2000], 4, 16, 2, 64, 32, 0), ([1500, 40], 1, 4, 2, 128, 16, 100),
     ([1500, 40, 3], 3, 9, 9, 64, 32, 500), ([900], 2, 6, 3, 128, 256, 1), ([31] * 40, 1, 4, 2, 64, 16, 0),
-    ([50, 2, 1], 8, 8, 1, 128, 16, 0), ([2100], 1, 2, 2, 64, 1024, 0),
+    ([50, 2, 1], 8, 8, 1, 128, 16, 0), ([4000, 200], 20, 8, 1, 128, 16, 0), ([3000], 100, 2, 2, 64, 16, 1000), ([2100], 1, 2, 2, 64, 1024, 0),
 ]  # fmt: skip
 
 
