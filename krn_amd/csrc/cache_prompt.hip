@@ -184,20 +184,28 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
     voff[i] = (uint32_t)(key * RB + v_slot<D>(in_tile, s) * 16);
   }
   const int shift = c.cache.page_shift;
-  // the page of this wave's group in tile u, or -1; without a branch, which would draw the work around it into its blocks
-  const auto page_of = [&](int u) {
-    const int at = ((first + u) * PROMPT_TILE + group * 16) >> shift;
-    const int number = ((const __attribute__((address_space(4))) int*)(uintptr_t)table)[max(0, min(at, c.s.width - 1))];
-    return u < n && at < c.s.width ? number : -1;
+  // page numbers of this wave's group in 64 tiles, a lane each
+  int ids = -1, ids_from = 0;
+  const auto fetch_ids = [&](int u) {
+    ids_from = u;
+    const int64_t at = ((int64_t)(first + u + lane) * PROMPT_TILE + group * 16) >> shift;
+    ids = u + lane < n && at < c.s.width ? table[at] : -1;
+    asm volatile("" : "+v"(ids));  // waited for here: a use in the loop would wait for the tiles on their way each time
   };
-  const auto load = [&](const void* data, int number, int u, int ring, const uint32_t(&off)[LOADS]) {
-    const int key0 = (first + u) * PROMPT_TILE + group * 16;
+  // where the group lies in tile u, and how many bytes the sequence has there
+  struct Group {
+    int64_t at;
+    int bytes;
+  };
+  const auto group_of = [&](int u) {
+    const int number = __builtin_amdgcn_readlane(ids, u - ids_from), key0 = (first + u) * PROMPT_TILE + group * 16;
     const bool there = (uint32_t)number < (uint32_t)c.cache.pages;
-    const int64_t at = ((((int64_t)(there ? number : 0) * c.kv_heads + column) << shift) + (key0 & ((1 << shift) - 1))) * RB;
-    const int bytes = __builtin_amdgcn_readfirstlane(there ? max(0, min(16, end - key0)) * RB : 0);
-    const __amdgpu_buffer_rsrc_t r = panel_rsrc((const uint8_t*)data + at, bytes);
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) buffer_to_lds16(r, lds + ring + wave * (TILE / 8) + i * 1024, off[i], 0);
+    const int64_t page = (int64_t)(there ? number : 0) * c.kv_heads + column;
+    return Group{((page << shift) + (key0 & ((1 << shift) - 1))) * RB,
+                 __builtin_amdgcn_readfirstlane(there ? max(0, min(16, end - key0)) * RB : 0)};
+  };
+  const auto load = [&](const void* data, const Group& g, int ring, const uint32_t(&off)[LOADS], int i) {
+    buffer_to_lds16(panel_rsrc((const uint8_t*)data + g.at, g.bytes), lds + ring + wave * (TILE / 8) + i * 1024, off[i], 0);
   };
   constexpr int V_RING = PROMPT_RING * TILE;
   const auto ring_of = [](int u) { return (u & (PROMPT_RING - 1)) * TILE; };
@@ -279,7 +287,8 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
   };
   // Tile u, whose exponents `s` are settled: the scores `next` of tile u + 1 beside most weights of u, then O += P V beside the
   // others and the exponents of u + 1. One MFMA and a little of the other work at a time, in this order.
-  const auto step = [&](f32x16(&s)[2], f32x16(&next)[2], int u, int& next_k, int& next_v) {
+  // K's tile u + 5 and V's u + 3 leave meanwhile; `at` says where the tiles u + 3 and u + 4 lie.
+  const auto step = [&](f32x16(&s)[2], f32x16(&next)[2], int u, Group(&at)[2]) {
     const uint32_t k_at = kat + ring_of(u + 1), k_then = kat + ring_of(u + 2), v_at = vat + ring_of(u);
     constexpr int FIRST = 24, SCORES = 2 * STEPS, PRODUCTS = 4 * BLOCKS;
     next[0] = f32x16{}, next[1] = f32x16{};
@@ -295,8 +304,6 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * LOADS) : "memory");  // this wave's part of K of u + 2 and V of u + 1
     KRN_BARRIER();
     __builtin_amdgcn_sched_barrier(0);
-    load(c.cache.values, next_v, u + 3, V_RING + ring_of(u + 3), voff);
-    load(c.cache.keys, next_k, u + 5, ring_of(u + 1), koff);
     float top[2] = {-INFINITY, -INFINITY};
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -310,24 +317,33 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
         for (int x = FIRST + i * (PIECES - FIRST) / LAST; x < FIRST + (i + 1) * (PIECES - FIRST) / LAST; ++x) piece(s, x);
 #pragma unroll
       for (int x = i * 16 / PRODUCTS; x < (i + 1) * 16 / PRODUCTS; ++x) scaled(next[x / 8], x % 8 * 2, top[x / 8]);
+      // a lane's addresses and loads here and there between the products: all at once they would hold them up
+      if (i < LOADS) load(c.cache.values, at[0], V_RING + ring_of(u + 3), voff, i);
+      if (i == PRODUCTS / 4) at[0] = at[1], at[1] = group_of(u + 5);
+      if (i >= PRODUCTS / 2 && i < PRODUCTS / 2 + LOADS) load(c.cache.keys, at[1], ring_of(u + 1), koff, i - PRODUCTS / 2);
       __builtin_amdgcn_sched_barrier(0);
     }
     asm volatile("" : "+v"(top[0]), "+v"(top[1]), "+v"(total));  // here, not in the branches that follow
-    next_v = page_of(u + 4), next_k = page_of(u + 6);
+    if (u + 6 - ids_from >= 64) fetch_ids(u + 6);
     settle(next, fmaxf(top[0], top[1]), u + 1);
   };
 
   // tiles on their way in the order that the loop keeps: V of u + 3, then K of u + 5
-  int k_page[6];
+  fetch_ids(0);
+  Group at[5];
 #pragma unroll
-  for (int u = 0; u < 6; ++u) k_page[u] = page_of(u);
-  load(c.cache.keys, k_page[0], 0, ring_of(0), koff);
-  load(c.cache.keys, k_page[1], 1, ring_of(1), koff);
-  load(c.cache.values, k_page[0], 0, V_RING + ring_of(0), voff);
-  load(c.cache.keys, k_page[2], 2, ring_of(2), koff);
-  load(c.cache.values, k_page[1], 1, V_RING + ring_of(1), voff);
-  load(c.cache.keys, k_page[3], 3, ring_of(3), koff);
-  load(c.cache.values, k_page[2], 2, V_RING + ring_of(2), voff);
+  for (int u = 0; u < 5; ++u) at[u] = group_of(u);
+  const auto load_tile = [&](const void* data, int u, int ring, const uint32_t(&off)[LOADS]) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) load(data, at[u], ring + ring_of(u), off, i);
+  };
+  load_tile(c.cache.keys, 0, 0, koff);
+  load_tile(c.cache.keys, 1, 0, koff);
+  load_tile(c.cache.values, 0, V_RING, voff);
+  load_tile(c.cache.keys, 2, 0, koff);
+  load_tile(c.cache.values, 1, V_RING, voff);
+  load_tile(c.cache.keys, 3, 0, koff);
+  load_tile(c.cache.values, 2, V_RING, voff);
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * LOADS) : "memory");  // the first two K tiles and the first V tile
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) asm volatile("" : "+v"(qf[s]));  // older loads: no wait for them in the loop
@@ -350,12 +366,12 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
   read_keys(kat + ring_of(1), 1);
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   KRN_BARRIER();  // everyone has read the first tile: its place may be loaded
-  load(c.cache.keys, k_page[4], 4, ring_of(0), koff);
-  int next_k = k_page[5], next_v = k_page[3];
+  load_tile(c.cache.keys, 4, 0, koff);
+  Group coming[2] = {at[3], at[4]};
   for (int u = 0;;) {
-    step(sa, sb, u, next_k, next_v);
+    step(sa, sb, u, coming);
     if (++u >= n) break;
-    step(sb, sa, u, next_k, next_v);
+    step(sb, sa, u, coming);
     if (++u >= n) break;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may reach LDS after the workgroup
