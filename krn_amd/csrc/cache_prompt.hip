@@ -27,34 +27,40 @@ constexpr int PROMPT_RING = 4;                          // tiles of K, and of V
 struct PromptTile {
   int seq, row0;
   TokenRange range;
+  int length;
 };
-__device__ __forceinline__ int64_t first_slot(const PromptCall& c, int i) {
-  const int start = min(max(c.s.starts[i], 0), c.s.tokens);
-  return (int64_t)start * c.group / PROMPT_ROWS + i;
+__device__ __forceinline__ int64_t slot_of(const PromptCall& c, int start, int i) {
+  return (int64_t)min(max(start, 0), c.s.tokens) * c.group / PROMPT_ROWS + i;
 }
 __device__ __forceinline__ bool find_tile(const PromptCall& c, int slot, PromptTile& tile) {
-  int seq, at;
+  int at;
   if (c.s.starts) {
     const int lane = threadIdx.x & 63;
     int low = 0, count = c.s.n;  // the last sequence of low to low + count - 1 whose first slot is this one or before
-    while (count > 1) {
-      const int step = (count + 63) / 64, i = lane * step;
-      const uint64_t before = __builtin_amdgcn_ballot_w64(i < count && first_slot(c, low + min(i, count - 1)) <= slot);
+    while (count > 64) {
+      const int step = (count + 63) / 64, i = low + min(lane * step, count - 1);
+      const uint64_t before = __builtin_amdgcn_ballot_w64(lane * step < count && slot_of(c, c.s.starts[i], i) <= slot);
       const int k = before ? 63 - __builtin_clzll(before) : 0;
       low += k * step;
       count = min(step, count - k * step);
     }
-    seq = __builtin_amdgcn_readfirstlane(low);
-    const int64_t from = slot - first_slot(c, seq);
+    // one more look, with what is needed of the sequence
+    const int i = low + min(lane, count - 1), start = c.s.starts[i], next = c.s.starts[i + 1], length = sequence_length(c.s, i);
+    const uint64_t before = __builtin_amdgcn_ballot_w64(lane < count && slot_of(c, start, i) <= slot);
+    const int k = __builtin_amdgcn_readfirstlane(before ? 63 - __builtin_clzll(before) : 0);
+    const int first = min(max(start, 0), c.s.tokens);
+    tile.seq = __builtin_amdgcn_readfirstlane(low) + k;
+    tile.range.first = __builtin_amdgcn_readlane(first, k);
+    tile.range.count = __builtin_amdgcn_readlane(min(max(next, first), c.s.tokens) - first, k);
+    tile.length = __builtin_amdgcn_readlane(length, k);
+    const int64_t from = slot - slot_of(c, tile.range.first, tile.seq);
     at = from < 0 || from > 0xffffff ? -1 : (int)from;
   } else {
     const int per = (c.s.step * c.group + PROMPT_ROWS - 1) / PROMPT_ROWS;
-    seq = slot / per, at = slot % per;
+    tile.seq = __builtin_amdgcn_readfirstlane(slot / per), at = slot - tile.seq * per;
+    tile.range = token_range(c.s, tile.seq);
+    tile.length = __builtin_amdgcn_readfirstlane(sequence_length(c.s, tile.seq));
   }
-  tile.seq = __builtin_amdgcn_readfirstlane(seq);
-  tile.range = token_range(c.s, tile.seq);
-  tile.range.first = __builtin_amdgcn_readfirstlane(tile.range.first);
-  tile.range.count = __builtin_amdgcn_readfirstlane(tile.range.count);
   at = __builtin_amdgcn_readfirstlane(at);
   tile.row0 = at * PROMPT_ROWS;
   return at >= 0 && (int64_t)at * PROMPT_ROWS < (int64_t)tile.range.count * c.group;
@@ -127,6 +133,7 @@ __device__ __forceinline__ bool find_part(const PromptCall& c, int w, bool write
   tile.range = token_range(c.s, tile.seq);
   tile.range.first = __builtin_amdgcn_readfirstlane(tile.range.first);
   tile.range.count = __builtin_amdgcn_readfirstlane(tile.range.count);
+  tile.length = __builtin_amdgcn_readfirstlane(sequence_length(c.s, tile.seq));
   before = (uint32_t)__builtin_amdgcn_readlane((int)before, of);
   share.parts = __builtin_amdgcn_readlane(parts, of), share.part = w - (int)(before & 0xffff), share.order = (int)(before >> 16);
   return share.parts > 0;  // always, where starts do not decrease
@@ -148,7 +155,7 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
   static_assert(LOADS >= 1, "whole loads a wave");
   const int t = threadIdx.x, lane = t & 63, half = lane >> 5, r32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int length = __builtin_amdgcn_readfirstlane(sequence_length(c.s, tile.seq));
+  const int length = tile.length;
   const int end = __builtin_amdgcn_readfirstlane(held_keys(c.s, length, c.cache.page_shift));
   const int before = length - tile.range.count;  // the position of the sequence's first token here
 
@@ -325,7 +332,7 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
     }
     asm volatile("" : "+v"(top[0]), "+v"(top[1]), "+v"(total));  // here, not in the branches that follow
     if (u + 6 - ids_from >= 64) fetch_ids(u + 6);
-    settle(next, fmaxf(top[0], top[1]), u + 1);
+    if (u + 1 < n) settle(next, fmaxf(top[0], top[1]), u + 1);  // no tile: its scores must not move the base
   };
 
   // tiles on their way in the order that the loop keeps: V of u + 3, then K of u + 5
@@ -344,7 +351,7 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
   load_tile(c.cache.values, 1, V_RING, voff);
   load_tile(c.cache.keys, 3, 0, koff);
   load_tile(c.cache.values, 2, V_RING, voff);
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * LOADS) : "memory");  // the first two K tiles and the first V tile
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(6 * LOADS) : "memory");  // the first K tile
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) asm volatile("" : "+v"(qf[s]));  // older loads: no wait for them in the loop
   KRN_BARRIER();
@@ -362,10 +369,10 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
     for (int x = 0; x < 16; ++x) scaled(sa[x / 8], x % 8 * 2, top);
     settle(sa, top, 0);
   }
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(4 * LOADS) : "memory");  // the second, and V's first
+  KRN_BARRIER();  // everyone has read the first tile: its place may be loaded
   read_keys(kat + ring_of(1), 0);
   read_keys(kat + ring_of(1), 1);
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  KRN_BARRIER();  // everyone has read the first tile: its place may be loaded
   load_tile(c.cache.keys, 4, 0, koff);
   Group coming[2] = {at[3], at[4]};
   for (int u = 0;;) {

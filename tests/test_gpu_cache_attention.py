@@ -178,6 +178,21 @@ def test_large_scores_and_infinite_ones(device, kind, packed):
     assert_within(got, y, bound)
 
 
+@pytest.mark.parametrize("packed,counts", [(True, [3]), (True, [200]), (False, [4]), (False, [100])])
+def test_scores_far_below_zero(device, packed, counts):
+    """Equal scores of -7200: the weights are equal, in every part that the keys are shared out to, but for roundings of exponents
+    of that size: 7200 * 2^-24 of a weight, in the maximum that it is taken from too, and for both once more where parts are
+    joined; values are at most 9."""
+    rng = np.random.default_rng(11)
+    paged = Paged(device, rng, "f16", [5000], kv_heads=1, d=64, fill=(lambda rng, shape: np.full(shape, -30.0), small))
+    starts = [0, *np.cumsum(counts).tolist()]
+    q = np.full((starts[-1], 2, 64), 30, np.float16)
+    sequences = paged.sequences(starts=starts) if packed else paged.sequences(new=counts[0])
+    got = values(cache_attention(paged.tensor(q), paged.cache, sequences))
+    y, _ = paged.attention(q.astype(np.float64), starts)
+    assert_within(got, y, 4 * 7200 * 2.0**-24 * 9 + np.abs(y) * 2 * HALF_STEP["f16"])
+
+
 @pytest.mark.parametrize("packed", [True, False])
 def test_nan_reaches_its_own_head_and_sequence_only(device, packed):
     rng = np.random.default_rng(6)
