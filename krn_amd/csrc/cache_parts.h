@@ -57,6 +57,9 @@ constexpr int TOKEN_WAVES = 4;
 constexpr int TOKEN_ROWS = 64;     // rows of a key head, at most; more are a prompt's
 constexpr int TOKEN_PARTS = 1024;  // parts that the keys of all sequences and columns are shared out to
 constexpr int TOKEN_CHUNK = 4;     // tiles of a part, at least
+// Tables of no more tiles a sequence keep each in one workgroup, which saves the joining launch (8 key heads, d = 128, one launch
+// and two: 300 keys 5.8 and 8.5 us, 256 sequences of 100 26.3 and 37.4, 16 of 200 8.7 and 10.5; 1000 keys 9.4 and 8.7)
+constexpr int TOKEN_WHOLE = 24;
 constexpr int TOKEN_SPLIT = 2048;  // sequences; more keep the keys of each in one workgroup
 constexpr int TOKEN_TILES = 1 << 20;  // of a sequence, as far as shares go by them: the sum of all stays below 2^32
 static_assert(TOKEN_PARTS + TOKEN_SPLIT < 1 << 16, "parts are counted in 16 bits");

@@ -451,7 +451,7 @@ TokenPlan krn::token_plan(int64_t step, int64_t group, int64_t kv_heads, int64_t
   p.shares = TOKEN_PARTS / p.columns;
   int64_t extra = p.shares;
   if (sequences * ((tiles - 1) / TOKEN_CHUNK) < extra) extra = sequences * ((tiles - 1) / TOKEN_CHUNK);
-  if (sequences > TOKEN_SPLIT) extra = 0;
+  if (sequences > TOKEN_SPLIT || tiles - 1 <= TOKEN_WHOLE) extra = 0;
   p.workgroups = sequences + extra;
   p.split = extra > 0;
   p.joins = sequences < extra ? sequences : extra;

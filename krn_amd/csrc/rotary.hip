@@ -4,14 +4,19 @@
 // Pair j of a head, (a, b), becomes m (a cos t - b sin t, b cos t + a sin t) with t = position * frequency[j]. The angle is
 // kept in turns as a 64-bit fraction: frequency / 2 pi mod 1 times 2^64, multiplied by the position modulo 2^64, is exact at
 // any position, where a float32 angle is off by 0.06 rad at a million. Its upper 32 bits go to sincospif as half turns. The
-// sines of a token serve all its heads, so a workgroup computes them once, into LDS.
+// sines of a token serve all its heads, so a workgroup has one token, or some heads of it, and computes them once, into LDS.
 //
 // Bound by memory: every byte of the projection is read once and written once, 16 bytes a lane.
 #include "cache_parts.h"
 
 namespace krn {
 
-constexpr int ROTARY_TOKENS = 4;  // of a workgroup, whose 256 threads then compute one sine each for 64 pairs
+// Workgroups, as far as the heads of few tokens fill them (32 query and 8 key heads of 128, one workgroup a token and this:
+// 16 tokens 7.4 and 3.5 us, 128 tokens 7.6 and 3.8)
+constexpr int ROTARY_SPREAD = 1024;
+// Bytes of a projection that is read non-temporally, half of the last-level cache: a larger one has left it by the time it is
+// read (192 MiB 76.7 and 65.5 us; 48 MiB, of which much is still there, 18.1 and 20.9)
+constexpr int64_t ROTARY_ONCE = (int64_t)128 << 20;
 
 // How a head's pairs lie: full halves or interleaved pairs in whole 16-byte chunks, or anything else, by elements
 enum RotaryForm : int { HALVES = 0, INTERLEAVED = 1, HALVES_ODD = 2, INTERLEAVED_ODD = 3 };
@@ -24,7 +29,7 @@ struct RotaryCall {
   const uint64_t* turns;
   int heads, rotary;
   float magnitude;
-  int parts;  // workgroups that share the heads of a token group
+  int parts;  // workgroups that share the heads of a token
 };
 
 template <bool BF>
@@ -48,111 +53,108 @@ __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
   return {narrow2<BF>(x[0], x[1]), narrow2<BF>(x[2], x[3]), narrow2<BF>(x[4], x[5]), narrow2<BF>(x[6], x[7])};
 }
 
-template <bool BF, int D, int FORM>
+template <bool BF, int D, int FORM, bool ONCE>
 __global__ __launch_bounds__(256) void rotary_append(RotaryCall c) {
-  __shared__ float2 turn[ROTARY_TOKENS][D / 2];  // cos and sin
-  __shared__ int owner[ROTARY_TOKENS], position[ROTARY_TOKENS];
-  __shared__ int64_t slot[ROTARY_TOKENS];  // the cache row of a token's first key head; negative: none
-  const int t = threadIdx.x, group = blockIdx.x / c.parts, part = blockIdx.x % c.parts;
-  const int first = group * ROTARY_TOKENS, count = min(ROTARY_TOKENS, c.s.tokens - first);
+  __shared__ float2 turn[D / 2];  // cos and sin
+  __shared__ int ended[4];
+  __shared__ int position;
+  __shared__ int64_t slot;  // the cache row of the token's first key head; negative: none; NOBODY: nor a query
+  constexpr int64_t NOBODY = -2;
+  const int t = threadIdx.x, token = blockIdx.x / c.parts, part = blockIdx.x % c.parts;
   const int kv = c.cache.kv_heads, page = 1 << c.cache.page_shift;
 
-  // the sequence of a token: how many sequences end at or before it
-  if (t < ROTARY_TOKENS) owner[t] = 0;
-  __syncthreads();
+  // the token's sequence: as many as end at or before it come first
+  int owner = 0;
   if (c.s.starts) {
-    int ended[ROTARY_TOKENS] = {};
-    for (int i = t + 1; i <= c.s.n; i += 256) {
-      const int start = c.s.starts[i];
+    int count = 0;
+    for (int i = t + 1; i <= c.s.n; i += 256) count += c.s.starts[i] <= token;
 #pragma unroll
-      for (int k = 0; k < ROTARY_TOKENS; ++k) ended[k] += start <= first + k;
-    }
-#pragma unroll
-    for (int k = 0; k < ROTARY_TOKENS; ++k)
-      if (ended[k]) atomicAdd(&owner[k], ended[k]);
+    for (int d = 1; d < 64; d *= 2) count += __shfl_xor(count, d);
+    if (t % 64 == 0) ended[t / 64] = count;
     __syncthreads();
-  } else if (t < count) {
-    owner[t] = (first + t) / c.s.step;
+    owner = ended[0] + ended[1] + ended[2] + ended[3];
+  } else {
+    owner = token / c.s.step;
   }
-  if (t < count) {
-    const int i = owner[t];
+  if (t == 0) {
     int at = 0;
-    bool mine = i < c.s.n;
-    int64_t row = -1;
-    if (mine) {
-      const TokenRange range = token_range(c.s, i);
-      mine = first + t >= range.first && first + t < range.first + range.count;
-      at = sequence_length(c.s, i) - (range.first + range.count - first - t);
+    int64_t row = NOBODY;
+    if (owner < c.s.n) {
+      const TokenRange range = token_range(c.s, owner);
+      at = sequence_length(c.s, owner) - (range.first + range.count - token);
+      if (token >= range.first && token < range.first + range.count) {
+        row = -1;
+        if (at >= 0 && (at >> c.cache.page_shift) < c.s.width) {
+          const int number = c.s.table[(int64_t)owner * c.s.width + (at >> c.cache.page_shift)];
+          if ((uint32_t)number < (uint32_t)c.cache.pages)
+            row = ((int64_t)number * kv << c.cache.page_shift) + (at & (page - 1));
+        }
+      }
     }
-    if (mine && at >= 0 && (at >> c.cache.page_shift) < c.s.width) {
-      const int number = c.s.table[(int64_t)i * c.s.width + (at >> c.cache.page_shift)];
-      if (number >= 0 && number < c.cache.pages)
-        row = ((int64_t)number * kv << c.cache.page_shift) + (at & (page - 1));
-    }
-    owner[t] = mine ? i : -1;
-    position[t] = at;
-    slot[t] = row;
+    position = at, slot = row;
   }
   __syncthreads();
+  if (slot == NOBODY) return;
   const int half = c.rotary / 2;
-  for (int u = t; u < count * half; u += 256) {
-    const int k = u / half, j = u % half;
-    const uint64_t angle = (uint64_t)(int64_t)position[k] * c.turns[j];
+  if (t < half) {
+    const uint64_t angle = (uint64_t)(int64_t)position * c.turns[t];
     float sin, cos;
     sincospif((float)(int32_t)(angle >> 32) * 0x1p-31f, &sin, &cos);
-    turn[k][j] = {cos * c.magnitude, sin * c.magnitude};
+    turn[t] = {cos * c.magnitude, sin * c.magnitude};
   }
   __syncthreads();
 
   // a rotated head is `units` pieces of work, a value head D / 8
   const int rotated = c.heads + kv, width = (rotated + kv) * D;
   const int units = FORM == HALVES ? c.rotary / 16 + (D - c.rotary) / 8 : D / 8;
-  const int per_token = rotated * units + kv * (D / 8);
-  const int begin = (int)((int64_t)per_token * count * part / c.parts),
-            end = (int)((int64_t)per_token * count * (part + 1) / c.parts);
+  const int pieces = rotated * units + kv * (D / 8);
+  const int begin = (int)((int64_t)pieces * part / c.parts), end = (int)((int64_t)pieces * (part + 1) / c.parts);
+  const auto read = [&](const uint16_t* at) {
+    const u32x4* x = reinterpret_cast<const u32x4*>(at);
+    if constexpr (ONCE) return __builtin_nontemporal_load(x);
+    else return *x;
+  };
   for (int u = begin + t; u < end; u += 256) {
-    const int k = u / per_token, item = u % per_token;
-    if (owner[k] < 0) continue;
-    const bool value = item >= rotated * units;
-    const int head = value ? rotated + (item - rotated * units) / (D / 8) : item / units;
-    const int unit = value ? (item - rotated * units) % (D / 8) : item % units;
-    const uint16_t* from = c.qkv + (int64_t)(first + k) * width + head * D;
+    const int over = u - rotated * units;
+    const bool value = over >= 0;
+    const int head = value ? rotated + over / (D / 8) : u / units, unit = value ? over % (D / 8) : u % units;
+    const uint16_t* from = c.qkv + (int64_t)token * width + head * D;
     uint16_t* to;
     if (head < c.heads) {
-      to = c.q + ((int64_t)(first + k) * c.heads + head) * D;
+      to = c.q + ((int64_t)token * c.heads + head) * D;
     } else {
-      if (slot[k] < 0) continue;
+      if (slot < 0) continue;
       const int h = value ? head - rotated : head - c.heads;
-      to = (value ? c.values : c.keys) + (slot[k] + ((int64_t)h << c.cache.page_shift)) * D;
+      to = (value ? c.values : c.keys) + (slot + ((int64_t)h << c.cache.page_shift)) * D;
     }
     if (value) {
-      *reinterpret_cast<u32x4*>(to + unit * 8) = *reinterpret_cast<const u32x4*>(from + unit * 8);
+      *reinterpret_cast<u32x4*>(to + unit * 8) = read(from + unit * 8);
     } else if (FORM == HALVES) {
       const int pairs = c.rotary / 16;
       if (unit >= pairs) {
         const int at = c.rotary + (unit - pairs) * 8;
-        *reinterpret_cast<u32x4*>(to + at) = *reinterpret_cast<const u32x4*>(from + at);
+        *reinterpret_cast<u32x4*>(to + at) = read(from + at);
         continue;
       }
       float a[8], b[8];
-      unpack8<BF>(*reinterpret_cast<const u32x4*>(from + unit * 8), a);
-      unpack8<BF>(*reinterpret_cast<const u32x4*>(from + half + unit * 8), b);
+      unpack8<BF>(read(from + unit * 8), a);
+      unpack8<BF>(read(from + half + unit * 8), b);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float2 w = turn[k][unit * 8 + e];
+        const float2 w = turn[unit * 8 + e];
         const float x = a[e] * w.x - b[e] * w.y, y = b[e] * w.x + a[e] * w.y;
         a[e] = x, b[e] = y;
       }
       *reinterpret_cast<u32x4*>(to + unit * 8) = pack8<BF>(a);
       *reinterpret_cast<u32x4*>(to + half + unit * 8) = pack8<BF>(b);
     } else if (FORM == INTERLEAVED) {
-      u32x4 w = *reinterpret_cast<const u32x4*>(from + unit * 8);
+      u32x4 w = read(from + unit * 8);
       if (unit * 8 < c.rotary) {
         float x[8];
         unpack8<BF>(w, x);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float2 z = turn[k][unit * 4 + e];
+          const float2 z = turn[unit * 4 + e];
           const float a = x[2 * e], b = x[2 * e + 1];
           x[2 * e] = a * z.x - b * z.y, x[2 * e + 1] = b * z.x + a * z.y;
         }
@@ -161,14 +163,14 @@ __global__ __launch_bounds__(256) void rotary_append(RotaryCall c) {
       *reinterpret_cast<u32x4*>(to + unit * 8) = w;
     } else {
       float x[8];
-      unpack8<BF>(*reinterpret_cast<const u32x4*>(from + unit * 8), x);
+      unpack8<BF>(read(from + unit * 8), x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int at = unit * 8 + e;
         if (at >= c.rotary) continue;
         const bool second = FORM == INTERLEAVED_ODD ? at & 1 : at >= half;
         const int other = FORM == INTERLEAVED_ODD ? at ^ 1 : second ? at - half : at + half;
-        const float2 z = turn[k][FORM == INTERLEAVED_ODD ? at / 2 : second ? other : at];
+        const float2 z = turn[FORM == INTERLEAVED_ODD ? at / 2 : second ? other : at];
         const float y = widen<BF>(from[other]);
         x[e] = x[e] * z.x + (second ? y * z.y : -(y * z.y));
       }
@@ -232,6 +234,18 @@ bool krn_cache_arguments(const CacheArguments& a, CacheView& cache, SequencesVie
   return true;
 }
 
+template <bool BF, int D, int FORM, bool ONCE>
+static void launch_form(const RotaryCall& c, hipStream_t stream) {
+  hipLaunchKernelGGL((rotary_append<BF, D, FORM, ONCE>), dim3((unsigned)((int64_t)c.s.tokens * c.parts)), dim3(256), 0, stream, c);
+}
+template <bool BF, int D>
+static void launch(const RotaryCall& c, RotaryForm form, bool once, hipStream_t stream) {
+  if (form == HALVES) once ? launch_form<BF, D, HALVES, true>(c, stream) : launch_form<BF, D, HALVES, false>(c, stream);
+  else if (form == INTERLEAVED) once ? launch_form<BF, D, INTERLEAVED, true>(c, stream) : launch_form<BF, D, INTERLEAVED, false>(c, stream);
+  else if (form == HALVES_ODD) launch_form<BF, D, HALVES_ODD, false>(c, stream);
+  else launch_form<BF, D, INTERLEAVED_ODD, false>(c, stream);
+}
+
 extern "C" int krn_rotary_append(int kind, const void* qkv, void* q, void* keys, void* values, int64_t tokens,
                                  int64_t heads, int64_t kv_heads, int64_t d, int64_t pages, int64_t page, const int* starts,
                                  int64_t step, const int* lengths, const int* table, int64_t sequences, int64_t width,
@@ -266,25 +280,13 @@ extern "C" int krn_rotary_append(int kind, const void* qkv, void* q, void* keys,
   if (tokens == 0 || sequences == 0) return 0;
   c.qkv = (const uint16_t*)qkv, c.q = (uint16_t*)q, c.keys = (uint16_t*)keys, c.values = (uint16_t*)values;
   c.turns = turns, c.heads = (int)heads, c.rotary = (int)rotary, c.magnitude = magnitude;
-  const int64_t groups = (tokens + ROTARY_TOKENS - 1) / ROTARY_TOKENS;
-  c.parts = 1;
+  const int64_t pieces = (heads + 2 * kv_heads) * (d / 8), spread = (ROTARY_SPREAD + tokens - 1) / tokens, most = (pieces + 255) / 256;
+  c.parts = (int)(spread < most ? spread : most);
   const bool whole = interleaved ? rotary % 8 == 0 : rotary % 16 == 0;
-  const int form = (interleaved ? INTERLEAVED : HALVES) + (whole ? 0 : 2);
-  const dim3 grid((unsigned)(groups * c.parts)), block(256);
-#define KRN_ROTARY(BF, D, FORM) hipLaunchKernelGGL((rotary_append<BF, D, FORM>), grid, block, 0, (hipStream_t)stream, c)
-#define KRN_ROTARY_FORMS(BF, D)                         \
-  switch (form) {                                       \
-    case HALVES: KRN_ROTARY(BF, D, HALVES); break;       \
-    case INTERLEAVED: KRN_ROTARY(BF, D, INTERLEAVED); break; \
-    case HALVES_ODD: KRN_ROTARY(BF, D, HALVES_ODD); break;   \
-    default: KRN_ROTARY(BF, D, INTERLEAVED_ODD);         \
-  }
-  if (kind == BF16 && d == 128) KRN_ROTARY_FORMS(true, 128)
-  else if (kind == BF16) KRN_ROTARY_FORMS(true, 64)
-  else if (d == 128) KRN_ROTARY_FORMS(false, 128)
-  else KRN_ROTARY_FORMS(false, 64)
-#undef KRN_ROTARY_FORMS
-#undef KRN_ROTARY
+  const RotaryForm form = interleaved ? whole ? INTERLEAVED : INTERLEAVED_ODD : whole ? HALVES : HALVES_ODD;
+  const bool once = in >= ROTARY_ONCE;
+  if (kind == BF16) d == 128 ? launch<true, 128>(c, form, once, (hipStream_t)stream) : launch<true, 64>(c, form, once, (hipStream_t)stream);
+  else d == 128 ? launch<false, 128>(c, form, once, (hipStream_t)stream) : launch<false, 64>(c, form, once, (hipStream_t)stream);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) {
     krn_set_error("rotary_append launch: %s", hipGetErrorString(err));
