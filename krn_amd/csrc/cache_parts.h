@@ -55,8 +55,11 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 // Attention of new tokens, a few of every sequence (cache_token.hip)
 constexpr int TOKEN_WAVES = 4;
 constexpr int TOKEN_ROWS = 64;     // rows of a key head, at most; more are a prompt's
-constexpr int TOKEN_PARTS = 1024;  // parts that the keys of all sequences and columns are shared out to
-constexpr int TOKEN_CHUNK = 4;     // tiles of a part, at least
+// Parts that the keys of all sequences and columns are shared out to: two for each workgroup that runs at once. (64 sequences of
+// 4096 keys on average, d = 128: 512 parts 179 us, 1024 173, 2048 176; of 4096 each 164, 170, 175; 2 of 131000 103, 99, 102.)
+constexpr int TOKEN_PARTS = 1024;
+// Tiles of a part, at least, one a wave (one sequence of 4096 keys 10.6 us, with 8 11.0, with 16 12.7)
+constexpr int TOKEN_CHUNK = 4;
 // Tables of no more tiles a sequence keep each in one workgroup, which saves the joining launch (8 key heads, d = 128, one launch
 // and two: 300 keys 5.8 and 8.5 us, 256 sequences of 100 26.3 and 37.4, 16 of 200 8.7 and 10.5; 1000 keys 9.4 and 8.7)
 constexpr int TOKEN_WHOLE = 24;
@@ -88,7 +91,9 @@ void launch_cache_tokens(bool bf, int d, TokenCall c, const TokenPlan& p, void* 
 // Attention of packed prompts (cache_prompt.hip)
 constexpr int PROMPT_ROWS = 256;  // of a workgroup: tokens times query heads of a key head
 
-constexpr int PROMPT_CHUNK = 16;  // tiles of 64 keys of a part, at least
+// Tiles of 64 keys of a part, at least: a part costs 133 KB of sums written and read (512 tokens after 15900, 28 heads on 4:
+// 363 us in one part, 140 in four; 128 after 8000, 32 on 8: 172 and 41)
+constexpr int PROMPT_CHUNK = 16;
 constexpr int PROMPT_CUS = 256;   // workgroups that run at once
 
 struct PromptCall {

@@ -14,7 +14,9 @@
 // are idle nine tenths of the time.
 //
 // K and V tiles come into LDS by direct loads, one buffer each a wave and no barrier: K's next tile leaves when this one's
-// fragments are in registers, V's likewise, so 8 to 16 KiB a wave are always on their way. Sixteen keys lie in one page,
+// fragments are in registers, V's likewise, so 8 to 16 KiB a wave are always on their way. The loads are non-temporal: a step
+// reads its whole cache before it reads a line again (196 us with plain ones, 176 with these; caches that stay in the last-level
+// cache between steps lose nothing: one sequence of 4096 keys 11.8 and 11.3). Sixteen keys lie in one page,
 // whose rows up to the sequence's end are a buffer resource: rows past it, and pages that are not there, read as zeros.
 #include "cache_parts.h"
 
