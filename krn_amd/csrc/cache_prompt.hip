@@ -5,12 +5,13 @@
 // its eight waves owns 32 rows and computes S^T = K Q^T and O^T += V^T P^T with 32x32x16 MFMAs: a lane holds one row
 // (lane & 31) and half of the keys (its partner is lane ^ 32), P stays in its lane.
 //
-// The matrix cores and the power that they draw bound it (16384 tokens, 32 heads of 128 on 8: 1.85 ms, 1190 TFLOP/s, the matrix
-// cores busy 61 % of the cycles at 1.77 GHz; a large library product reaches 1380). Two waves share a SIMD. Each interleaves its own
-// work: scores of the next tile beside the weights of this one, then O += P V beside the exponents of the next, one MFMA and a few
-// other instructions at a time in the order written (left to the compiler, 2 % slower; waves taking
-// turns by barriers instead, one group's products beside the other's weights, 2.06 ms). Four waves of 64 rows, which halve
-// the LDS reads, need more than 256 registers for what vector instructions touch, and their copies made 2.27 ms.
+// The matrix cores and the power that they draw bound it (16384 tokens, 32 heads of 128 on 8: 1.84 ms, 1195 TFLOP/s, the
+// matrix cores busy 61 % of the cycles at 1.77 GHz; a large library product reaches 1380). Two waves share a SIMD. Each
+// interleaves its own work: scores of the next tile beside the weights of this one, then O += P V beside the exponents of the
+// next, one MFMA and a few other instructions at a time in the order written (left to the compiler, 2 % slower; waves taking
+// turns by barriers instead, one group's products beside the other's weights, 2.06 ms). Four waves of 64 rows halve the LDS
+// reads, but need more than 256 registers: 2.27 ms with the compiler's copies from and to the accumulation registers, 2.04
+// with accumulators that products alone touch.
 //
 // K and V come into rings of four tiles by direct loads, four tiles and three ahead of their use, so that a wait finds them
 // there; tiles past the end are asked for with no bytes, which keeps the count of loads on their way the same. Sixteen
@@ -24,11 +25,11 @@
 
 namespace krn {
 
-constexpr int PROMPT_TILE = 64;                         // keys
-constexpr int PROMPT_RING = 4;                          // tiles of K, and of V
+constexpr int PROMPT_TILE = 64;  // keys
+constexpr int PROMPT_RING = 4;   // tiles of K, and of V
 
-// The tokens of slot `slot`: 256 rows of a sequence. Sequence i has the slots from first_slot(i) on, enough for its rows since
-// starts are sums of what came before; a wave looks at 64 sequences at a time.
+// The tokens of slot `slot`: 256 rows of a sequence. Sequence i has the slots from slot_of(its start, i) on, enough for its
+// rows since starts are sums of what came before; a wave looks at 64 sequences at a time.
 struct PromptTile {
   int seq, row0;
   TokenRange range;

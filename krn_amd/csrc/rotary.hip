@@ -14,8 +14,9 @@ namespace krn {
 // Workgroups, as far as the heads of few tokens fill them (32 query and 8 key heads of 128, one workgroup a token and this:
 // 16 tokens 7.4 and 3.5 us, 128 tokens 7.6 and 3.8)
 constexpr int ROTARY_SPREAD = 1024;
-// Bytes of a projection that is read non-temporally, half of the last-level cache: a larger one has left it by the time it is
-// read (192 MiB 76.7 and 65.5 us; 48 MiB, of which much is still there, 18.1 and 20.9)
+// Bytes of a projection that is read and written non-temporally, half of the last-level cache: neither a larger one nor its
+// results stay there (192 MiB 76.9 and 67.9 us, and with the product before and the attention behind it 766 and 758). Of a
+// smaller one much does (48 MiB 21.4 and 17.8 us by itself, 104.4 and 106.1 in that company)
 constexpr int64_t ROTARY_ONCE = (int64_t)128 << 20;
 
 // How a head's pairs lie: full halves or interleaved pairs in whole 16-byte chunks, or anything else, by elements
@@ -114,6 +115,11 @@ __global__ __launch_bounds__(256) void rotary_append(RotaryCall c) {
     if constexpr (ONCE) return __builtin_nontemporal_load(x);
     else return *x;
   };
+  const auto write = [&](uint16_t* at, u32x4 w) {
+    u32x4* x = reinterpret_cast<u32x4*>(at);
+    if constexpr (ONCE) __builtin_nontemporal_store(w, x);
+    else *x = w;
+  };
   for (int u = begin + t; u < end; u += 256) {
     const int over = u - rotated * units;
     const bool value = over >= 0;
@@ -128,12 +134,12 @@ __global__ __launch_bounds__(256) void rotary_append(RotaryCall c) {
       to = (value ? c.values : c.keys) + (slot + ((int64_t)h << c.cache.page_shift)) * D;
     }
     if (value) {
-      *reinterpret_cast<u32x4*>(to + unit * 8) = read(from + unit * 8);
+      write(to + unit * 8, read(from + unit * 8));
     } else if (FORM == HALVES) {
       const int pairs = c.rotary / 16;
       if (unit >= pairs) {
         const int at = c.rotary + (unit - pairs) * 8;
-        *reinterpret_cast<u32x4*>(to + at) = read(from + at);
+        write(to + at, read(from + at));
         continue;
       }
       float a[8], b[8];
@@ -145,8 +151,8 @@ __global__ __launch_bounds__(256) void rotary_append(RotaryCall c) {
         const float x = a[e] * w.x - b[e] * w.y, y = b[e] * w.x + a[e] * w.y;
         a[e] = x, b[e] = y;
       }
-      *reinterpret_cast<u32x4*>(to + unit * 8) = pack8<BF>(a);
-      *reinterpret_cast<u32x4*>(to + half + unit * 8) = pack8<BF>(b);
+      write(to + unit * 8, pack8<BF>(a));
+      write(to + half + unit * 8, pack8<BF>(b));
     } else if (FORM == INTERLEAVED) {
       u32x4 w = read(from + unit * 8);
       if (unit * 8 < c.rotary) {
@@ -160,7 +166,7 @@ __global__ __launch_bounds__(256) void rotary_append(RotaryCall c) {
         }
         w = pack8<BF>(x);
       }
-      *reinterpret_cast<u32x4*>(to + unit * 8) = w;
+      write(to + unit * 8, w);
     } else {
       float x[8];
       unpack8<BF>(read(from + unit * 8), x);
@@ -174,7 +180,7 @@ __global__ __launch_bounds__(256) void rotary_append(RotaryCall c) {
         const float y = widen<BF>(from[other]);
         x[e] = x[e] * z.x + (second ? y * z.y : -(y * z.y));
       }
-      *reinterpret_cast<u32x4*>(to + unit * 8) = pack8<BF>(x);
+      write(to + unit * 8, pack8<BF>(x));
     }
   }
 }
