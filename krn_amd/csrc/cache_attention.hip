@@ -48,7 +48,7 @@ extern "C" int krn_cache_attention(int kind, const void* q, const void* keys, co
     krn_set_error("cache_attention: a window of %lld keys", (long long)window);
     return -1;
   }
-  if (tokens * heads > 0x7fffffff) {
+  if (tokens * heads > 0x7fffffff - PROMPT_ROWS) {
     krn_set_error("cache_attention: %lld tokens of %lld heads", (long long)tokens, (long long)heads);
     return -1;
   }

@@ -37,6 +37,40 @@ __device__ __forceinline__ int first_key(int position, int window) {
   return window ? (int)max((int64_t)0, (int64_t)position + 1 - window) : 0;
 }
 
+// Values that are not finite: a weight of zero does not make them zero. Where a tile has keys that some rows see and some do
+// not, the products take its values without those, and each row adds the ones that it sees: its sum is not finite either way.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+template <bool BF>
+constexpr uint32_t ENDLESS = BF ? 0x7f80 : 0x7c00;  // infinity; NaN are above
+template <bool BF, int N>
+__device__ __forceinline__ bool any_endless(const u32x4 (&w)[N]) {
+  u16x2 top = {};
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i][e] & 0x7fff7fffu));
+  return top[0] >= ENDLESS<BF> || top[1] >= ENDLESS<BF>;
+}
+template <bool BF>
+__device__ __forceinline__ u32x4 without_endless(u32x4 w) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if ((w[e] & 0x7fff) >= ENDLESS<BF>) w[e] &= 0xffff0000u;
+    if ((w[e] >> 16 & 0x7fff) >= ENDLESS<BF>) w[e] &= 0xffffu;
+  }
+  return w;
+}
+template <bool BF>
+__device__ __forceinline__ f32x4 only_endless(u32x2 w) {
+  f32x4 x;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint16_t v = (uint16_t)(w[e / 2] >> (e % 2 * 16));
+    x[e] = (v & 0x7fff) >= ENDLESS<BF> ? (BF ? bf2f(v) : h2f(v)) : 0.0f;
+  }
+  return x;
+}
+
 // The sum over lanes up to this one: rows of sixteen by shifts, then the rows' ends
 template <int CTRL, int ROWS>
 __device__ __forceinline__ uint32_t from_lane(uint32_t x) {

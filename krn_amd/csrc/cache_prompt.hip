@@ -170,6 +170,10 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
   const bool real = j < tile.range.count;
   const int limit = min(before + min(j, tile.range.count - 1) + 1, end), low = first_key(before + min(j, tile.range.count - 1), c.window);
   const int all_limit = __builtin_amdgcn_readfirstlane(limit), all_low = __builtin_amdgcn_readlane(low, 31);
+  // tiles within these bounds have keys that all rows of the workgroup see, or that lie past the end and are zeros
+  const int last_token = min((tile.row0 + PROMPT_ROWS - 1) / c.group, tile.range.count - 1);
+  const int whole_low = __builtin_amdgcn_readfirstlane(first_key(before + last_token, c.window));
+  const int whole_limit = __builtin_amdgcn_readfirstlane(min(before + tile.row0 / c.group + 1, end));
   const KeyTiles seen = tiles_seen(c, tile.range, length, tile.row0);
   const int even = __builtin_amdgcn_readfirstlane(seen.count / parts), over = seen.count - even * parts;
   const int first = __builtin_amdgcn_readfirstlane(seen.first + even * part + min(part, over));
@@ -298,12 +302,49 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
       margin = moves ? 8.0f : margin;
     }
   };
+  // Tile u has keys that some rows see and some do not: if values of it are not finite, which every wave looks for in what it
+  // loaded, all of them add what their rows see of those and clear them away. (The look costs 1 % of 12 prompts of 8192 tokens,
+  // 3 % of 16 of 500. It comes before the step's products: beside them the compiler would move weights behind its branch, and
+  // behind them copy the sums.)
+  const auto separate = [&](int u) {
+    u32x4* mine = reinterpret_cast<u32x4*>(lds + V_RING + ring_of(u) + wave * (TILE / 8)) + lane;
+    uint32_t* flags = reinterpret_cast<uint32_t*>(lds + 2 * V_RING);  // a wave each
+    u32x4 held[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) held[i] = mine[i * 64];
+    flags[wave] = __builtin_amdgcn_ballot_w64(any_endless<BF>(held)) != 0;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    KRN_BARRIER();
+    if (__builtin_amdgcn_ballot_w64(flags[lane & 7] != 0) != 0) {
+#pragma unroll 1
+      for (int k = 0; k < PROMPT_TILE; ++k) {
+        const int key = (first + u) * PROMPT_TILE + k;
+        const bool sees = key >= low && key < limit;
+#pragma unroll
+        for (int i = 0; i < BLOCKS; ++i)
+#pragma unroll
+          for (int gq = 0; gq < 4; ++gq) {
+            const f32x4 v = only_endless<BF>(*reinterpret_cast<const u32x2*>(
+                lds + V_RING + ring_of(u) + k * RB + v_slot<D>(k, i * 4 + gq) * 16 + half * 8));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][gq * 4 + e] += sees ? v[e] : 0.0f;
+          }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      KRN_BARRIER();
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) mine[i * 64] = without_endless<BF>(mine[i * 64]);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      KRN_BARRIER();
+    }
+  };
   // Tile u, whose exponents `s` are settled: the scores `next` of tile u + 1 beside most weights of u, then O += P V beside the
   // others and the exponents of u + 1. One MFMA and a little of the other work at a time, in this order.
   // K's tile u + 5 and V's u + 3 leave meanwhile; `at` says where the tiles u + 3 and u + 4 lie.
   const auto step = [&](f32x16(&s)[2], f32x16(&next)[2], int u, Group(&at)[2]) {
     const uint32_t k_at = kat + ring_of(u + 1), k_then = kat + ring_of(u + 2), v_at = vat + ring_of(u);
     constexpr int FIRST = 24, SCORES = 2 * STEPS, PRODUCTS = 4 * BLOCKS;
+    if ((first + u) * PROMPT_TILE < whole_low || min((first + u + 1) * PROMPT_TILE, end) > whole_limit) separate(u);
     next[0] = f32x16{}, next[1] = f32x16{};
 #pragma unroll
     for (int i = 0; i < SCORES; ++i) {
@@ -434,7 +475,7 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
 
 template <bool BF, int D>
 __global__ __launch_bounds__(512, 2) void cache_prompt(PromptCall c) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * PROMPT_RING * PROMPT_TILE * D * 2];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * PROMPT_RING * PROMPT_TILE * D * 2 + 8 * 4];
   const int w = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / c.kv_heads)), column = (int)blockIdx.x - w * c.kv_heads;
   PromptTile tile;
   PromptPart share{0, 1, 0};

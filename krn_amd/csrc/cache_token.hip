@@ -270,15 +270,12 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES, NB < 4 ? 2 : 1) void cache_tokens
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) acc[b][i] = f32x4{};
   }
-  if (first < last) {
-    fetch_ids(first);
+  if (first < last) fetch_ids(first);
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+  for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int s = 0; s < D / 32; ++s) asm volatile("" : "+v"(qf[b][s]));  // here too, for the same reason
-    load_keys(first);
-    load_values();
-  }
+    for (int s = 0; s < D / 32; ++s) asm volatile("" : "+v"(qf[b][s]));  // here too, for the same reason
+  if (first < last) load_keys(first), load_values();
   for (int tile = first; tile < last; ++tile) {
     const bool more = tile + 1 < last;
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory");  // K is here, V may be on its way
@@ -333,6 +330,27 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES, NB < 4 ? 2 : 1) void cache_tokens
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory");  // V is here, the next K may be on its way
     else
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (tile * 32 < all_low || min(tile * 32 + 32, end) > all_limit) {  // keys that some rows see and some do not
+      u32x4* here = reinterpret_cast<u32x4*>(vbuf) + lane;
+      u32x4 held[TILE / 1024];
+#pragma unroll
+      for (int i = 0; i < TILE / 1024; ++i) held[i] = here[i * 64];
+      if (__builtin_amdgcn_ballot_w64(any_endless<BF>(held)) != 0) {
+#pragma unroll 1
+        for (int k = 0; k < 32; ++k)
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            const f32x4 v = only_endless<BF>(
+                *reinterpret_cast<const u32x2*>(vbuf + k * RB + value_chunk<D>(k % 16, i * 2 + g / 2) * 16 + g % 2 * 8));
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+              if (tile * 32 + k < limit[b] && tile * 32 + k >= low[b]) acc[b][i] += v;
+          }
+#pragma unroll
+        for (int i = 0; i < TILE / 1024; ++i) here[i * 64] = without_endless<BF>(held[i]);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+    }
 #pragma unroll
     for (int q = 0; q < D / 64; ++q) {
       u32x4 vf[4];

@@ -212,6 +212,58 @@ def test_nan_reaches_its_own_head_and_sequence_only(device, packed):
     assert np.all(np.abs(got - y)[~bad] <= bound[~bad])
 
 
+# packed or new tokens each, lengths, counts of new tokens, heads, kv_heads, d, page, window
+UNSEEN = [
+    (True, [100], [90], 4, 2, 128, 16, 0), (True, [500, 31], [300, 31], 8, 2, 64, 32, 0), (True, [3040], [40], 4, 1, 128, 16, 0),
+    (True, [600, 40], [200, 31], 8, 2, 128, 32, 100), (True, [513], [313], 1, 1, 64, 16, 33), (True, [2000], [60], 6, 2, 64, 64, 900),
+    (False, [70, 300], [4, 4], 4, 2, 128, 16, 0), (False, [3000], [8], 8, 1, 64, 32, 0), (False, [1500, 90], [1, 1], 4, 2, 128, 16, 100),
+    (False, [1500], [20], 9, 3, 64, 16, 37), (False, [400], [100], 4, 4, 64, 32, 70),
+]  # fmt: skip
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("packed,lengths,counts,heads,kv_heads,d,page,window", UNSEEN)
+def test_what_a_token_does_not_see_does_not_reach_it(device, kind, packed, lengths, counts, heads, kv_heads, d, page, window):
+    """NaN and infinities in some of the new keys and values, in a column of theirs or a head, and in all that lies before the
+    first window, whose pages may be another sequence's by then. A token that sees none of them gets what it gets without."""
+    rng = np.random.default_rng(12)
+    paged = Paged(device, rng, kind, lengths, kv_heads=kv_heads, d=d, page=page)
+    starts, group = [0, *np.cumsum(counts).tolist()], heads // kv_heads
+    bad = np.zeros((starts[-1], heads, d), bool)
+    put = []
+    for i, (length, count) in enumerate(zip(lengths, counts)):
+        positions = np.arange(length - count, length)
+        lows = np.maximum(0, positions + 1 - window) if window else 0 * positions
+        at = lambda k: (paged.table[i, k // page], slice(None), k % page)  # noqa: B023, E731
+        for k in range(lows[0]):
+            put += [(paged.keys, at(k), np.nan), (paged.values, at(k), rng.choice([np.nan, np.inf, -np.inf]))]
+        some = np.arange(1 + (lows if window else positions)[0], length)  # not all tokens see these
+        for n, k in enumerate(sorted(rng.choice(some, min(5, len(some)), replace=False))):
+            page_, _, row = at(k)
+            head, col = rng.integers(kv_heads), rng.integers(d)
+            sees = (starts[i] + np.flatnonzero((positions >= k) & (lows <= k)))[:, None]
+            of_head = np.arange(head * group, (head + 1) * group)
+            if n == 3:
+                put.append((paged.keys, (page_, head, row), np.nan))
+                bad[sees, of_head] = True
+            else:
+                put.append((paged.values, (page_, head, row, col), [np.nan, np.inf, -np.inf][n % 3]))
+                bad[sees, of_head, col] = True
+    assert 0 < bad.sum() < bad.size
+    for data, where, value in put:
+        data[where] = value
+    with np.errstate(invalid="ignore"):
+        cache = KvCache(paged.tensor(words(paged.keys, kind)[0]), paged.tensor(words(paged.values, kind)[0]))
+    for data, where, _ in put:
+        data[where] = 0
+    q, exact = words(rng.standard_normal((starts[-1], heads, d)), kind)
+    sequences = paged.sequences(starts=starts) if packed else paged.sequences(new=counts[0])
+    got = values(cache_attention(paged.tensor(q), cache, sequences, window=window or None))
+    y, bound = paged.attention(exact, starts, window=window)
+    np.testing.assert_array_equal(~np.isfinite(got), bad)
+    assert np.all(np.abs(got - y)[~bad] <= bound[~bad])
+
+
 @pytest.mark.parametrize("packed", [True, False])
 @pytest.mark.parametrize("scale", [1e-30, 0.01, 3.0])
 def test_scales(device, packed, scale):
