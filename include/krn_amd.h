@@ -183,8 +183,8 @@ int64_t krn_moe_workspace(int kind, int64_t tokens, int64_t hidden, int64_t inne
 
 /* A paged key-value cache: `keys` and `values` are each pages x kv_heads x page x d, of kind KRN_F16 or KRN_BF16, d 64 or 128,
  * page a power of two from 16 to 65536, 16-byte aligned. The sequences of a step: `lengths` (sequences) counts the keys of each,
- * those of its newest tokens included, and `table` (sequences x width) numbers the pages that it owns: key j of sequence i lies
- * in row j % page of page table[i, j / page]. The step's tokens are packed; those of sequence i are starts[i] to
+ * those of its newest tokens included, and `table` (sequences x width, width * page below 2^31 - 255) numbers the pages that it
+ * owns: key j of sequence i lies in row j % page of page table[i, j / page]. The step's tokens are packed; those of sequence i are starts[i] to
  * starts[i + 1] - 1 (`starts` has sequences + 1 entries and does not decrease) or, with starts NULL, `step` for every sequence
  * (tokens = step * sequences). Its last token has position lengths[i] - 1. All three arrays are int32 on the device and are read
  * when the kernels run. They are checked there: a token that no range holds belongs to no sequence and what would be written

@@ -219,6 +219,11 @@ bool krn_cache_arguments(const CacheArguments& a, CacheView& cache, SequencesVie
     krn_set_error("%s: at most 2^31 - 1 pages of 2^40 keys in all, 2^23 - 1 sequences and as many tokens", a.name);
     return false;
   }
+  if (a.width > 0x7fffff00 / a.page) {  // key numbers, rounded up to a tile, are 32-bit
+    krn_set_error("%s: tables of %lld pages of %lld keys; fewer than 2^31 - 255 keys a sequence", a.name, (long long)a.width,
+                  (long long)a.page);
+    return false;
+  }
   if (!a.starts && (a.step < 1 || a.step > 0x7fffff || a.tokens != a.step * a.sequences)) {
     krn_set_error("%s: %lld tokens are not %lld for each of %lld sequences", a.name, (long long)a.tokens, (long long)a.step,
                   (long long)a.sequences);

@@ -207,6 +207,7 @@ def test_the_entry_points_refuse_before_any_device_call():
         for sizes in ({"pages": 1 << 31}, {"pages": 1 << 30, "page": 2048}, {"width": 1 << 31}, {"sequences": 1 << 23, "tokens": 1 << 23},
                       {"tokens": 1 << 23, "starts": 1 << 24}):
             assert "at most" in refused(name, **sizes)
+        assert "a sequence" in refused(name, width=(1 << 27) - 15) and "a sequence" in refused(name, width=1 << 15, page=1 << 16, pages=1)
         assert "are not" in refused(name, tokens=4) and "are not" in refused(name, step=0) and "are not" in refused(name, step=-1)
         assert "cache must be" in refused(name, keys=(1 << 41) + 8) and "cache must be" in refused(name, values=(1 << 42) + 2)
         for what in ("lengths", "table"):
