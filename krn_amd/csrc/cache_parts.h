@@ -123,12 +123,12 @@ TokenPlan token_plan(int64_t step, int64_t group, int64_t kv_heads, int64_t d, i
 void launch_cache_tokens(bool bf, int d, TokenCall c, const TokenPlan& p, void* workspace, hipStream_t stream);
 
 // Attention of packed prompts (cache_prompt.hip)
-constexpr int PROMPT_ROWS = 256;  // of a workgroup: tokens times query heads of a key head
+constexpr int PROMPT_ROWS = 128;  // of a workgroup: tokens times query heads of a key head
 
-// Tiles of 64 keys of a part, at least: a part costs 133 KB of sums written and read (512 tokens after 15900, 28 heads on 4:
-// 363 us in one part, 140 in four; 128 after 8000, 32 on 8: 172 and 41)
+// Tiles of 64 keys of a part, at least: a part costs 67 KB of sums written and read (128 tokens after 8000, 32 heads on 8: 35.0 us,
+// with 8 40.9, with 32 43.4)
 constexpr int PROMPT_CHUNK = 16;
-constexpr int PROMPT_CUS = 256;   // workgroups that run at once
+constexpr int PROMPT_CUS = 512;   // workgroups that run at once
 
 struct PromptCall {
   const uint16_t* q;
@@ -140,7 +140,7 @@ struct PromptCall {
   int slots;        // workgroups of a key head without parts
   uint32_t shares;  // workgroups of a key head with parts, or 0
   int4* header;     // the number of tiles of rows in several parts, then of each (sequence, first row, first workgroup, parts)
-  float* planes;    // of a workgroup: 256 rows of sums, then their bases and sums of weights
+  float* planes;    // of a workgroup: PROMPT_ROWS rows of sums, then their bases and sums of weights
 };
 // slots: tiles of rows of a key head, without starts those of `step` tokens a sequence, else enough for any lengths (step 0)
 struct PromptPlan {

@@ -1,22 +1,22 @@
 // Causal attention of packed prompts over a paged cache, for rows enough to fill the matrix cores.
 //
-// A workgroup has 256 rows of one key head: row r of a sequence is its token r / group, query head r % group of the key head's
-// `group`. So shared heads lie side by side, short prompts fill tiles, and a causal tile is 256 / group tokens wide. Each of
-// its eight waves owns 32 rows and computes S^T = K Q^T and O^T += V^T P^T with 32x32x16 MFMAs: a lane holds one row
+// A workgroup has 128 rows of one key head: row r of a sequence is its token r / group, query head r % group of the key head's
+// `group`. So shared heads lie side by side, short prompts fill tiles, and a causal tile is 128 / group tokens wide. Each of
+// its four waves owns 32 rows and computes S^T = K Q^T and O^T += V^T P^T with 32x32x16 MFMAs: a lane holds one row
 // (lane & 31) and half of the keys (its partner is lane ^ 32), P stays in its lane.
 //
-// The matrix cores and the power that they draw bound it (16384 tokens, 32 heads of 128 on 8: 1.84 ms, 1195 TFLOP/s, the
-// matrix cores busy 61 % of the cycles at 1.77 GHz; a large library product reaches 1380). Two waves share a SIMD. Each
-// interleaves its own work: scores of the next tile beside the weights of this one, then O += P V beside the exponents of the
-// next, one MFMA and a few other instructions at a time in the order written (left to the compiler, 2 % slower; waves taking
-// turns by barriers instead, one group's products beside the other's weights, 2.06 ms). Four waves of 64 rows halve the LDS
-// reads, but need more than 256 registers: 2.27 ms with the compiler's copies from and to the accumulation registers, 2.04
-// with accumulators that products alone touch.
+// The matrix cores and the power that they draw bound it (16384 tokens, 32 heads of 128 on 8: 1.87 to 1.96 ms by the card, 1120
+// to 1180 TFLOP/s; a large library product reaches 1380). Two workgroups share a CU, two waves a SIMD. Each wave interleaves its
+// own work: scores of the next tile beside the weights of this one, then O += P V beside the exponents of the next, one MFMA
+// and a few other instructions at a time in the order written (left to the compiler, 2 % slower). The other workgroup covers
+// what comes before and after the loop: one workgroup of eight waves a CU reads keys half as often and has 0 to 2 % on that one prompt,
+// 5 on 512 tokens after 15900, but 12 prompts of 8192 tokens take 153 us in place of 144, 16 of 500 10.0 and 8.5, 1024 tokens 29.0
+// and 22.5. (Eight waves in two groups that take turns by barriers: 2.06 ms. Four of 64 rows halve the LDS reads, but need more
+// than 256 registers: 2.27 ms with the compiler's copies, 2.04 with accumulators that products alone touch.)
 //
-// K and V come into rings of four tiles by direct loads, four tiles and three ahead of their use, so that a wait finds them
-// there; tiles past the end are asked for with no bytes, which keeps the count of loads on their way the same. Sixteen
-// keys lie in one page, whose rows up to the sequence's end are a buffer resource: rows past it, and pages that are not
-// there, read as zeros.
+// K and V come into rings of three and two tiles by direct loads, more than a tile ahead of their use; tiles past the end are
+// asked for with no bytes, which keeps the count of loads on their way the same. Sixteen keys, a wave's part of a tile, lie in
+// one page, whose rows up to the sequence's end are a buffer resource: rows past it, and pages that are not there, read as zeros.
 //
 // Weights are rounded to 16 bits before O += P V, half a step (2^-8 in bf16) of each, as in attention.hip: two parts of them, which
 // cache_token.hip can afford, would be half as many products again.
@@ -26,9 +26,10 @@
 namespace krn {
 
 constexpr int PROMPT_TILE = 64;  // keys
-constexpr int PROMPT_RING = 4;   // tiles of K, and of V
+constexpr int PROMPT_WAVES = PROMPT_ROWS / 32;
+constexpr int PROMPT_KEYS = 3, PROMPT_VALUES = 2;  // tiles of each in their rings
 
-// The tokens of slot `slot`: 256 rows of a sequence. Sequence i has the slots from slot_of(its start, i) on, enough for its
+// The tokens of slot `slot`: 128 rows of a sequence. Sequence i has the slots from slot_of(its start, i) on, enough for its
 // rows since starts are sums of what came before; a wave looks at 64 sequences at a time.
 struct PromptTile {
   int seq, row0;
@@ -72,7 +73,7 @@ __device__ __forceinline__ bool find_tile(const PromptCall& c, int slot, PromptT
   return at >= 0 && (int64_t)at * PROMPT_ROWS < (int64_t)tile.range.count * c.group;
 }
 
-// The key tiles that 256 rows from row0 on see: from the first row's window to the last row's position
+// The key tiles that 128 rows from row0 on see: from the first row's window to the last row's position
 struct KeyTiles {
   int first, count;
 };
@@ -157,8 +158,9 @@ __device__ __forceinline__ bool find_part(const PromptCall& c, int w, bool write
 template <bool BF, int D>
 __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTile& tile, int column, int part, int parts,
                                             float* plane, const int* __restrict__ table, uint8_t* lds) {
-  constexpr int RB = D * 2, DCH = D / 8, TILE = PROMPT_TILE * RB, LOADS = TILE / 8 / 1024, STEPS = D / 16, BLOCKS = D / 32;
-  static_assert(LOADS >= 1, "whole loads a wave");
+  constexpr int RB = D * 2, DCH = D / 8, TILE = PROMPT_TILE * RB, LOADS = TILE / PROMPT_WAVES / 1024;
+  constexpr int STEPS = D / 16, BLOCKS = D / 32;
+  static_assert(PROMPT_TILE == PROMPT_WAVES * 16, "sixteen keys a wave");
   const int t = threadIdx.x, lane = t & 63, half = lane >> 5, r32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int length = tile.length;
@@ -190,47 +192,47 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) qf[s] = real ? *reinterpret_cast<const u32x4*>(c.q + place + s * 16 + half * 8) : u32x4{};
 
-  // this wave's eight keys of a tile, half of a group of sixteen
-  const int group = wave >> 1;
+  // this wave's sixteen keys of a tile
   uint32_t koff[LOADS], voff[LOADS];
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
-    const int key = (wave & 1) * 8 + i * (1024 / RB) + lane / DCH, s = lane % DCH;  // in the group
-    const int in_tile = group * 16 + key;
+    const int key = i * (1024 / RB) + lane / DCH, s = lane % DCH;  // in the group
+    const int in_tile = wave * 16 + key;
     koff[i] = (uint32_t)(key * RB + k_slot<D>(in_tile, s) * 16);
     voff[i] = (uint32_t)(key * RB + v_slot<D>(in_tile, s) * 16);
   }
   const int shift = c.cache.page_shift;
-  // page numbers of this wave's group in 64 tiles, a lane each
+  // page numbers of this wave's keys in 64 tiles, a lane each
   int ids = -1, ids_from = 0;
   const auto fetch_ids = [&](int u) {
     ids_from = u;
-    const int64_t at = ((int64_t)(first + u + lane) * PROMPT_TILE + group * 16) >> shift;
+    const int64_t at = ((int64_t)(first + u + lane) * PROMPT_TILE + wave * 16) >> shift;
     ids = u + lane < n && at < c.s.width ? table[at] : -1;
     asm volatile("" : "+v"(ids));  // waited for here: a use in the loop would wait for the tiles on their way each time
   };
-  // where the group lies in tile u, and how many bytes the sequence has there
+  // where they lie in tile u, and how many bytes the sequence has there
   struct Group {
     int64_t at;
     int bytes;
   };
   const auto group_of = [&](int u) {
-    const int number = __builtin_amdgcn_readlane(ids, u - ids_from), key0 = (first + u) * PROMPT_TILE + group * 16;
+    const int number = __builtin_amdgcn_readlane(ids, u - ids_from), key0 = (first + u) * PROMPT_TILE + wave * 16;
     const bool there = (uint32_t)number < (uint32_t)c.cache.pages;
     const int64_t page = (int64_t)(there ? number : 0) * c.kv_heads + column;
     return Group{((page << shift) + (key0 & ((1 << shift) - 1))) * RB,
                  __builtin_amdgcn_readfirstlane(there ? max(0, min(16, end - key0)) * RB : 0)};
   };
   const auto load = [&](const void* data, const Group& g, int ring, const uint32_t(&off)[LOADS], int i) {
-    buffer_to_lds16(panel_rsrc((const uint8_t*)data + g.at, g.bytes), lds + ring + wave * (TILE / 8) + i * 1024, off[i], 0);
+    buffer_to_lds16(panel_rsrc((const uint8_t*)data + g.at, g.bytes), lds + ring + wave * (TILE / PROMPT_WAVES) + i * 1024, off[i], 0);
   };
-  constexpr int V_RING = PROMPT_RING * TILE;
-  const auto ring_of = [](int u) { return (u & (PROMPT_RING - 1)) * TILE; };
+  constexpr int V_RING = PROMPT_KEYS * TILE;
+  const auto key_ring = [](int u) { return u % PROMPT_KEYS * TILE; };
+  const auto value_ring = [](int u) { return V_RING + u % PROMPT_VALUES * TILE; };
 
   // fragments: K's as A operands (lane = key, 8 columns of step s), V^T's (lane = column, keys as the lane's P has them)
   const uint32_t kat = r32 * RB + k_slot<D>(r32, half) * 16;
   const int a16 = lane & 15, tr_key = (lane >> 5) * 4 + (a16 >> 2), tr_col = ((lane >> 4) & 1) * 16 + 4 * (a16 & 3);
-  const uint32_t vat = V_RING + tr_key * RB + v_slot<D>(tr_key, tr_col >> 3) * 16 + (tr_col & 7) * 2;
+  const uint32_t vat = tr_key * RB + v_slot<D>(tr_key, tr_col >> 3) * 16 + (tr_col & 7) * 2;
   constexpr int K_AHEAD = 3, V_AHEAD = 2;  // steps whose fragments are held
   u32x4 kf[K_AHEAD][2], vf[V_AHEAD][BLOCKS];
   const auto read_keys = [&](uint32_t at, int s) {
@@ -303,19 +305,21 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
     }
   };
   // Tile u has keys that some rows see and some do not: if values of it are not finite, which every wave looks for in what it
-  // loaded, all of them add what their rows see of those and clear them away. (The look costs 1 % of 12 prompts of 8192 tokens,
-  // 3 % of 16 of 500. It comes before the step's products: beside them the compiler would move weights behind its branch, and
-  // behind them copy the sums.)
+  // loaded, all of them add what their rows see of those and clear them away. (The look costs 1 % of prompts of some hundred
+  // tokens. It comes before the step's products: beside them the compiler would move weights behind its branch, and behind
+  // them copy the sums.)
   const auto separate = [&](int u) {
-    u32x4* mine = reinterpret_cast<u32x4*>(lds + V_RING + ring_of(u) + wave * (TILE / 8)) + lane;
-    uint32_t* flags = reinterpret_cast<uint32_t*>(lds + 2 * V_RING);  // a wave each
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");  // this wave's part of V of u
+    KRN_BARRIER();
+    u32x4* mine = reinterpret_cast<u32x4*>(lds + value_ring(u) + wave * (TILE / PROMPT_WAVES)) + lane;
+    uint32_t* flags = reinterpret_cast<uint32_t*>(lds + value_ring(u + 1));  // a wave each: that tile comes in this step
     u32x4 held[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) held[i] = mine[i * 64];
     flags[wave] = __builtin_amdgcn_ballot_w64(any_endless<BF>(held)) != 0;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     KRN_BARRIER();
-    if (__builtin_amdgcn_ballot_w64(flags[lane & 7] != 0) != 0) {
+    if (__builtin_amdgcn_ballot_w64(flags[lane & (PROMPT_WAVES - 1)] != 0) != 0) {
 #pragma unroll 1
       for (int k = 0; k < PROMPT_TILE; ++k) {
         const int key = (first + u) * PROMPT_TILE + k;
@@ -325,7 +329,7 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
 #pragma unroll
           for (int gq = 0; gq < 4; ++gq) {
             const f32x4 v = only_endless<BF>(*reinterpret_cast<const u32x2*>(
-                lds + V_RING + ring_of(u) + k * RB + v_slot<D>(k, i * 4 + gq) * 16 + half * 8));
+                lds + value_ring(u) + k * RB + v_slot<D>(k, i * 4 + gq) * 16 + half * 8));
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[i][gq * 4 + e] += sees ? v[e] : 0.0f;
           }
@@ -340,26 +344,28 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
   };
   // Tile u, whose exponents `s` are settled: the scores `next` of tile u + 1 beside most weights of u, then O += P V beside the
   // others and the exponents of u + 1. One MFMA and a little of the other work at a time, in this order.
-  // K's tile u + 5 and V's u + 3 leave meanwhile; `at` says where the tiles u + 3 and u + 4 lie.
-  const auto step = [&](f32x16(&s)[2], f32x16(&next)[2], int u, Group(&at)[2]) {
-    const uint32_t k_at = kat + ring_of(u + 1), k_then = kat + ring_of(u + 2), v_at = vat + ring_of(u);
+  // Once every wave has K's fragments of u + 1, and V of u is there, V's tile u + 1 and K's u + 4 leave; `at` says where the
+  // tiles u + 1, u + 2 and u + 3 lie.
+  const auto step = [&](f32x16(&s)[2], f32x16(&next)[2], int u, Group(&at)[3]) {
+    const uint32_t k_at = kat + key_ring(u + 1), k_then = kat + key_ring(u + 2), v_at = vat + value_ring(u);
     constexpr int FIRST = 24, SCORES = 2 * STEPS, PRODUCTS = 4 * BLOCKS;
     if ((first + u) * PROMPT_TILE < whole_low || min((first + u + 1) * PROMPT_TILE, end) > whole_limit) separate(u);
     next[0] = f32x16{}, next[1] = f32x16{};
 #pragma unroll
     for (int i = 0; i < SCORES; ++i) {
       if (i % 2 == 0 && i / 2 + 2 < STEPS) read_keys(k_at, i / 2 + 2);
+      if (i == SCORES - BLOCKS) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");  // this wave's part of K of u + 2 and V of u
+        KRN_BARRIER();
+        __builtin_amdgcn_sched_barrier(0);
+      }
       if (i >= SCORES - BLOCKS) read_values(v_at, 0, i - (SCORES - BLOCKS));
       Half<BF>::mma(next[i % 2], kf[i / 2 % K_AHEAD][i % 2], qf[i / 2]);
 #pragma unroll
       for (int x = i * FIRST / SCORES; x < (i + 1) * FIRST / SCORES; ++x) piece(s, x);
       __builtin_amdgcn_sched_barrier(0);
     }
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * LOADS) : "memory");  // this wave's part of K of u + 2 and V of u + 1
-    KRN_BARRIER();
-    __builtin_amdgcn_sched_barrier(0);
     float top[2] = {-INFINITY, -INFINITY};
-    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < PRODUCTS; ++i) {
       if (i / BLOCKS < 3) read_values(v_at, i / BLOCKS + 1, i % BLOCKS);
@@ -372,33 +378,29 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
 #pragma unroll
       for (int x = i * 16 / PRODUCTS; x < (i + 1) * 16 / PRODUCTS; ++x) scaled(next[x / 8], x % 8 * 2, top[x / 8]);
       // a lane's addresses and loads here and there between the products: all at once they would hold them up
-      if (i < LOADS) load(c.cache.values, at[0], V_RING + ring_of(u + 3), voff, i);
-      if (i == PRODUCTS / 4) at[0] = at[1], at[1] = group_of(u + 5);
-      if (i >= PRODUCTS / 2 && i < PRODUCTS / 2 + LOADS) load(c.cache.keys, at[1], ring_of(u + 1), koff, i - PRODUCTS / 2);
+      if (i < LOADS) load(c.cache.values, at[0], value_ring(u + 1), voff, i);
+      if (i == PRODUCTS / 4) at[0] = at[1], at[1] = at[2], at[2] = group_of(u + 4);
+      if (i >= PRODUCTS / 2 && i < PRODUCTS / 2 + LOADS) load(c.cache.keys, at[2], key_ring(u + 1), koff, i - PRODUCTS / 2);
       __builtin_amdgcn_sched_barrier(0);
     }
     asm volatile("" : "+v"(top[0]), "+v"(top[1]), "+v"(total));  // here, not in the branches that follow
-    if (u + 6 - ids_from >= 64) fetch_ids(u + 6);
+    if (u + 5 - ids_from >= 64) fetch_ids(u + 5);
     if (u + 1 < n) settle(next, fmaxf(top[0], top[1]), u + 1);  // no tile: its scores must not move the base
   };
 
-  // tiles on their way in the order that the loop keeps: V of u + 3, then K of u + 5
+  // tiles on their way in the order that the loop keeps: V of u + 1, then K of u + 4
   fetch_ids(0);
-  Group at[5];
+  Group at[4];
 #pragma unroll
-  for (int u = 0; u < 5; ++u) at[u] = group_of(u);
-  const auto load_tile = [&](const void* data, int u, int ring, const uint32_t(&off)[LOADS]) {
+  for (int u = 0; u < 4; ++u) at[u] = group_of(u);
+  const auto load_keys = [&](int u) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) load(data, at[u], ring + ring_of(u), off, i);
+    for (int i = 0; i < LOADS; ++i) load(c.cache.keys, at[u], key_ring(u), koff, i);
   };
-  load_tile(c.cache.keys, 0, 0, koff);
-  load_tile(c.cache.keys, 1, 0, koff);
-  load_tile(c.cache.values, 0, V_RING, voff);
-  load_tile(c.cache.keys, 2, 0, koff);
-  load_tile(c.cache.values, 1, V_RING, voff);
-  load_tile(c.cache.keys, 3, 0, koff);
-  load_tile(c.cache.values, 2, V_RING, voff);
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(6 * LOADS) : "memory");  // the first K tile
+  load_keys(0), load_keys(1), load_keys(2);
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) load(c.cache.values, at[0], value_ring(0), voff, i);
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * LOADS) : "memory");  // the first K tile
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) asm volatile("" : "+v"(qf[s]));  // older loads: no wait for them in the loop
   KRN_BARRIER();
@@ -416,12 +418,12 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
     for (int x = 0; x < 16; ++x) scaled(sa[x / 8], x % 8 * 2, top);
     settle(sa, top, 0);
   }
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(4 * LOADS) : "memory");  // the second, and V's first
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * LOADS) : "memory");  // the second
   KRN_BARRIER();  // everyone has read the first tile: its place may be loaded
-  read_keys(kat + ring_of(1), 0);
-  read_keys(kat + ring_of(1), 1);
-  load_tile(c.cache.keys, 4, 0, koff);
-  Group coming[2] = {at[3], at[4]};
+  read_keys(kat + key_ring(1), 0);
+  read_keys(kat + key_ring(1), 1);
+  load_keys(3);
+  Group coming[3] = {at[1], at[2], at[3]};
   for (int u = 0;;) {
     step(sa, sb, u, coming);
     if (++u >= n) break;
@@ -474,8 +476,8 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
 #undef KRN_BARRIER
 
 template <bool BF, int D>
-__global__ __launch_bounds__(512, 2) void cache_prompt(PromptCall c) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * PROMPT_RING * PROMPT_TILE * D * 2 + 8 * 4];
+__global__ __launch_bounds__(64 * PROMPT_WAVES, 2) void cache_prompt(PromptCall c) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[(PROMPT_KEYS + PROMPT_VALUES) * PROMPT_TILE * D * 2];
   const int w = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / c.kv_heads)), column = (int)blockIdx.x - w * c.kv_heads;
   PromptTile tile;
   PromptPart share{0, 1, 0};
@@ -540,7 +542,7 @@ PromptPlan krn::prompt_plan(int64_t tokens, int64_t step, int64_t group, int64_t
 
 template <bool BF, int D>
 static void launch(const PromptCall& c, const PromptPlan& p, hipStream_t stream) {
-  hipLaunchKernelGGL((cache_prompt<BF, D>), dim3((unsigned)(p.workgroups * c.kv_heads)), dim3(512), 0, stream, c);
+  hipLaunchKernelGGL((cache_prompt<BF, D>), dim3((unsigned)(p.workgroups * c.kv_heads)), dim3(64 * PROMPT_WAVES), 0, stream, c);
   if (p.shares)
     hipLaunchKernelGGL((cache_prompt_join<BF, D>), dim3((unsigned)(p.joins * (PROMPT_ROWS * (D / 4) / 256) * c.kv_heads)),
                        dim3(256), 0, stream, c);
