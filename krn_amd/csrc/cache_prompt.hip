@@ -505,17 +505,16 @@ __global__ __launch_bounds__(256) void cache_prompt_join(PromptCall c) {
   if (j >= range.count) return;
   const int64_t stride = (int64_t)c.kv_heads * (PROMPT_ROWS * (D + 2));
   const float* plane = c.planes + head.z * stride + (int64_t)column * (PROMPT_ROWS * (D + 2));
-  float top = -INFINITY;
-  for (int p = 0; p < head.w; ++p) top = fmaxf(top, plane[p * stride + PROMPT_ROWS * D + r * 2]);
-  const float to_base = top == -INFINITY ? 0.0f : top;
-  float all = 0.0f;
+  float m = -INFINITY, all = 0.0f;
   f32x4 o = f32x4{};
 #pragma unroll 4
   for (int p = 0; p < head.w; ++p) {
     const float* at = plane + p * stride;
-    const float f = __builtin_amdgcn_exp2f(at[PROMPT_ROWS * D + r * 2] - to_base);
-    all += f * at[PROMPT_ROWS * D + r * 2 + 1];
-    o += f * *reinterpret_cast<const f32x4*>(at + r * D + d);
+    const float top = at[PROMPT_ROWS * D + r * 2], next = fmaxf(m, top), to_base = next == -INFINITY ? 0.0f : next;
+    const float f = __builtin_amdgcn_exp2f(m - to_base), h = __builtin_amdgcn_exp2f(top - to_base);
+    all = all * f + at[PROMPT_ROWS * D + r * 2 + 1] * h;
+    o = o * f + h * *reinterpret_cast<const f32x4*>(at + r * D + d);
+    m = next;
   }
   const float inv = all == 0.0f ? 0.0f : 1.0f / all;  // no key: zeros
   const u32x2 y = {Half<BF>::pack(o[0] * inv, o[1] * inv), Half<BF>::pack(o[2] * inv, o[3] * inv)};
