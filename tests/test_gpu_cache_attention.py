@@ -288,6 +288,33 @@ def test_a_result_over_its_queries(device, packed):
     assert_within(values(held), *paged.attention(exact, starts))
 
 
+@pytest.mark.parametrize("packed,n", [(True, 2), (True, 20), (True, 64), (True, 65), (False, 20), (False, 64)])
+def test_more_rows_than_run_at_once_are_those_of_each_sequence_alone(device, packed, n):
+    """Workgroups may take rows in any order: every row is the same to the last bit, and the others stay as they were."""
+    rng = np.random.default_rng(n)
+    counts = np.array([4000, 2500]) if n == 2 else rng.integers(0, 12000 // n, n) if packed else np.full(n, 100)
+    if packed and n > 2:
+        counts[3], counts[n - 1] = 0, 1
+    lengths = [int(c + b) for c, b in zip(counts, rng.integers(0, 400, n))]
+    if not packed:
+        lengths[2], lengths[5] = 30, 0  # fewer keys than new tokens
+    paged = Paged(device, rng, "bf16", lengths, kv_heads=16, d=64)
+    starts = [2, *(2 + np.cumsum(counts)).tolist()] if packed else [0, *np.cumsum(counts).tolist()]
+    tokens = starts[-1] + (3 if packed else 0)
+    q, _ = words(rng.standard_normal((tokens, 32, 64)), "bf16")
+    out = paged.tensor(np.full((tokens, 32, 64), 0x4040, np.uint16))
+    cache_attention(paged.tensor(q), paged.cache, paged.sequences(starts=starts) if packed else paged.sequences(new=100), out=out)
+    got = out.to_host()
+    assert (got[: starts[0]] == 0x4040).all() and (got[starts[-1] :] == 0x4040).all()
+    for i in range(n):
+        rows = slice(starts[i], starts[i + 1])
+        if counts[i] == 0:
+            continue
+        one = Sequences(device.to_device(np.array(lengths[i : i + 1], np.int32)), device.to_device(paged.table[i : i + 1].copy()),
+                        starts=device.to_device(np.array([0, counts[i]], np.int32)))
+        np.testing.assert_array_equal(got[rows], cache_attention(paged.tensor(q[rows].copy()), paged.cache, one).to_host())
+
+
 def test_nothing_to_attend(device):
     paged = Paged(device, np.random.default_rng(1), "bf16", [], kv_heads=1, d=64)
     empty = device.empty(BF16, 0, 3, 64)
