@@ -128,7 +128,11 @@ constexpr int PROMPT_ROWS = 128;  // of a workgroup: tokens times query heads of
 // Tiles of 64 keys of a part, at least: a part costs 67 KB of sums written and read (128 tokens after 8000, 32 heads on 8: 35.0 us,
 // with 8 40.9, with 32 43.4)
 constexpr int PROMPT_CHUNK = 16;
-constexpr int PROMPT_CUS = 512;   // workgroups that run at once
+// Tiles of a table, beyond which rows are shared out where they fill the chip as well: a single token before 65000 keys, packed
+// with a prompt of 2000 tokens, would run on alone (891 us, shared out 131). Counting parts and the joining launch cost 60
+// prompts of 150 tokens with such a table 53.6 and 59.1.
+constexpr int PROMPT_LONG = 128;
+constexpr int PROMPT_CUS = 512;  // workgroups that run at once
 
 struct PromptCall {
   const uint16_t* q;
@@ -139,12 +143,13 @@ struct PromptCall {
   float scale;                         // of the scores, times log2(e)
   int slots;        // workgroups of a key head without parts
   uint32_t shares;  // workgroups of a key head with parts, or 0
-  int4* header;     // the number of tiles of rows in several parts, then of each (sequence, first row, first workgroup, parts)
-  float* planes;    // of a workgroup: PROMPT_ROWS rows of sums, then their bases and sums of weights
+  uint32_t spare;   // those of them that parts beyond the first may take
+  int4* header;     // the number of tiles of rows in several parts, then of each (sequence, first row, first plane, parts)
+  float* planes;    // of a part: PROMPT_ROWS rows of sums, then their bases and sums of weights
 };
 // slots: tiles of rows of a key head, without starts those of `step` tokens a sequence, else enough for any lengths (step 0)
 struct PromptPlan {
-  int64_t slots, shares, workgroups, joins, header_bytes, bytes;
+  int64_t slots, shares, spare, workgroups, joins, header_bytes, bytes;
 };
 PromptPlan prompt_plan(int64_t tokens, int64_t step, int64_t group, int64_t kv_heads, int64_t d, int64_t page, int64_t sequences,
                        int64_t width, int64_t bytes);

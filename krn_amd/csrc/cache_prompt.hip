@@ -84,66 +84,84 @@ __device__ __forceinline__ KeyTiles tiles_seen(const PromptCall& c, const TokenR
   return {first, max(0, (max(end, 0) + PROMPT_TILE - 1) / PROMPT_TILE - first)};
 }
 
-// The key tiles of few tiles of rows are shared out: workgroup w of a column does part `part` of `parts` of some rows, the
-// `order`-th of those in several parts. A part has at most chunk tiles, chunk such that the parts fill the chip once: with S shares of a
-// column and R tiles of rows, T / (S - R). Every wave counts for itself, a lane for ceil(n / 64) sequences in a row.
+// Rows before many keys are shared out: workgroup w of a column does part `part` of `parts` of a tile of rows. All tiles of rows of a
+// sequence have as many parts, so that nothing loops over them: with R of them of up to T key tiles each, ceil(T / chunk), and chunk
+// is the sum of all R T over `spare`, the workgroups that are there beyond one for each tile of rows. Every wave counts
+// for itself, a lane for ceil(n / 64) sequences in a row. What no chip does in a second stays whole, and the sums below 2^32.
 struct PromptPart {
-  int part, parts, order;
+  int part, parts, plane, order;  // plane: of the first part, among all planes; order: of the rows, among those in several parts
 };
 __device__ __forceinline__ bool find_part(const PromptCall& c, int w, bool writes, PromptTile& tile, PromptPart& share) {
+  constexpr uint32_t MOST = 1 << 22;
   const int lane = threadIdx.x & 63, per = (c.s.n + 63) / 64, from = lane * per, to = min(from + per, c.s.n);
-  const auto weight_of = [&](const TokenRange& r, int length, int k) {  // capped: the sum of all stays below 2^32
-    return (uint32_t)min(tiles_seen(c, r, length, k * PROMPT_ROWS).count, 1 << 23);
+  struct Rows {
+    uint32_t rows, tiles;  // tiles of rows, and the key tiles of the last one
   };
-  const auto rows_of = [&](const TokenRange& r) { return (r.count * c.group + PROMPT_ROWS - 1) / PROMPT_ROWS; };
-  uint32_t tiles = 0, items = 0;
-  for (int i = from; i < to; ++i) {
-    const TokenRange range = token_range(c.s, i);
-    const int length = sequence_length(c.s, i), rows = rows_of(range);
-    items += rows;
-    for (int k = 0; k < rows; ++k) tiles += weight_of(range, length, k);
+  const auto rows_of = [&](const TokenRange& range, int length) {
+    const uint32_t rows = (range.count * c.group + PROMPT_ROWS - 1) / PROMPT_ROWS;
+    int first = 0;
+    if (c.window) first = first_key(length - range.count + (int)(rows - 1) * PROMPT_ROWS / c.group, c.window) / PROMPT_TILE;
+    const int end = held_keys(c.s, length, c.cache.page_shift);
+    return Rows{rows, rows ? (uint32_t)max((end + PROMPT_TILE - 1) / PROMPT_TILE - first, 1) : 0};
+  };
+  const auto work_of = [&](const Rows& r) { return (uint64_t)r.tiles * r.rows > MOST ? 0 : r.tiles * r.rows; };
+  // a lane's first sequence stays in registers
+  const int own = min(from, c.s.n - 1);
+  const TokenRange range = token_range(c.s, own);
+  const int length = sequence_length(c.s, own);
+  const Rows held = from < to ? rows_of(range, length) : Rows{0, 0};
+  uint32_t work = work_of(held), items = held.rows;
+  for (int i = from + 1; i < to; ++i) {
+    const Rows r = rows_of(token_range(c.s, i), sequence_length(c.s, i));
+    work += work_of(r), items += r.rows;
   }
-  tiles = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(tiles), 63);
-  items = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(items), 63);
-  const uint32_t spare = items < c.shares ? c.shares - items : 1;
-  const uint32_t chunk = items < c.shares ? max((uint32_t)PROMPT_CHUNK, (tiles + spare - 1) / spare) : 0x7fffffff;
-  // parts in the low half, rows in several of them in the high one
-  uint32_t count = 0;
-  for (int i = from; i < to; ++i) {
-    const TokenRange range = token_range(c.s, i);
-    const int length = sequence_length(c.s, i), rows = rows_of(range);
-    for (int k = 0; k < rows; ++k) {
-      const uint32_t parts = max(1u, (weight_of(range, length, k) + chunk - 1) / chunk);
-      count += parts + (parts > 1 ? 0x10000u : 0u);
-    }
+  uint32_t upto = wave_scan(items), before = upto - items;
+  work = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(work), 63);
+  const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+  const uint32_t spare = all < c.shares ? min(c.shares - all, c.spare) : 0;
+  const uint32_t chunk = spare ? max((uint32_t)PROMPT_CHUNK, (work + spare - 1) / spare) : 0x7fffffff;
+  const auto parts_of = [&](const Rows& r) {
+    return r.tiles <= chunk || (uint64_t)r.tiles * r.rows > MOST ? 1u : (r.tiles + chunk - 1) / chunk;
+  };
+  // parts, and of rows in several of them the parts in the low half, the rows in the high one
+  const uint32_t parts = parts_of(held);
+  uint32_t count = held.rows * parts, joined = parts > 1 ? held.rows << 16 | count : 0;
+  for (int i = from + 1; i < to; ++i) {
+    const Rows r = rows_of(token_range(c.s, i), sequence_length(c.s, i));
+    const uint32_t p = parts_of(r);
+    count += r.rows * p, joined += p > 1 ? r.rows << 16 | r.rows * p : 0;
   }
-  const uint32_t upto = wave_scan(count), all = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
-  if (writes && w == 0 && threadIdx.x == 0) c.header[0] = {items < c.shares ? (int)(all >> 16) : 0, 0, 0, 0};
-  uint32_t before = upto - count;
-  const uint64_t owner = __builtin_amdgcn_ballot_w64((int)(before & 0xffff) <= w && w < (int)(upto & 0xffff));
+  uint32_t joined_upto = 0;
+  if (__builtin_amdgcn_ballot_w64(joined != 0) != 0) {
+    upto = wave_scan(count), before = upto - count;
+    joined_upto = wave_scan(joined);
+  }
+  if (writes && w == 0 && threadIdx.x == 63) c.header[0] = {(int)(joined_upto >> 16), 0, 0, 0};
+  const uint64_t owner = __builtin_amdgcn_ballot_w64(before <= (uint32_t)w && (uint32_t)w < upto);
   if (owner == 0) return false;
-  int seq = 0, at = 0, parts = 0;
-  for (int i = from; i < to && parts == 0; ++i) {  // in the owner's lane: the rows
-    const TokenRange range = token_range(c.s, i);
-    const int length = sequence_length(c.s, i), rows = rows_of(range);
-    for (int k = 0; k < rows; ++k) {
-      const int p = (int)max(1u, (weight_of(range, length, k) + chunk - 1) / chunk);
-      if (w < (int)(before & 0xffff) + p) {
-        seq = i, at = k, parts = p;
-        break;
-      }
-      before += p + (p > 1 ? 0x10000u : 0u);
-    }
+  // in the owner's lane: the sequence
+  uint32_t joined_before = joined_upto - joined, at = (uint32_t)w - before;
+  Rows r = held;
+  uint32_t p = parts;
+  int seq = from;
+  while (at >= r.rows * p && seq + 1 < to) {
+    at -= r.rows * p, joined_before += p > 1 ? r.rows << 16 | r.rows * p : 0;
+    ++seq;
+    r = rows_of(token_range(c.s, seq), sequence_length(c.s, seq)), p = parts_of(r);
   }
+  const uint32_t row = p > 1 ? at / p : at;  // late rows, the long ones, first
+  joined_before += p > 1 ? row << 16 | row * p : 0;
   const int of = __builtin_ctzll(owner);
-  tile.seq = __builtin_amdgcn_readlane(seq, of), tile.row0 = __builtin_amdgcn_readlane(at, of) * PROMPT_ROWS;
-  tile.range = token_range(c.s, tile.seq);
-  tile.range.first = __builtin_amdgcn_readfirstlane(tile.range.first);
-  tile.range.count = __builtin_amdgcn_readfirstlane(tile.range.count);
-  tile.length = __builtin_amdgcn_readfirstlane(sequence_length(c.s, tile.seq));
-  before = (uint32_t)__builtin_amdgcn_readlane((int)before, of);
-  share.parts = __builtin_amdgcn_readlane(parts, of), share.part = w - (int)(before & 0xffff), share.order = (int)(before >> 16);
-  return share.parts > 0;  // always, where starts do not decrease
+  const auto get = [&](auto x) { return __builtin_amdgcn_readlane((int)x, of); };
+  share.part = get(at - row * p), share.parts = get(p), share.plane = get(joined_before & 0xffff), share.order = get(joined_before >> 16);
+  tile.seq = get(seq), tile.row0 = get(r.rows - 1 - row) * PROMPT_ROWS;
+  if (tile.seq == of * per) {
+    tile.range = {get(range.first), get(range.count)}, tile.length = get(length);
+  } else {
+    const TokenRange other = token_range(c.s, tile.seq);
+    tile.range = {get(other.first), get(other.count)}, tile.length = get(sequence_length(c.s, tile.seq));
+  }
+  return tile.row0 >= 0;
 }
 
 #define KRN_BARRIER()                       \
@@ -480,15 +498,20 @@ __global__ __launch_bounds__(64 * PROMPT_WAVES, 2) void cache_prompt(PromptCall 
   __shared__ __attribute__((aligned(1024))) uint8_t lds[(PROMPT_KEYS + PROMPT_VALUES) * PROMPT_TILE * D * 2];
   const int w = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / c.kv_heads)), column = (int)blockIdx.x - w * c.kv_heads;
   PromptTile tile;
-  PromptPart share{0, 1, 0};
+  PromptPart share{0, 1, 0, 0};
   if (c.shares) {
     if (!find_part(c, w, column == 0, tile, share)) return;
-    if (share.parts > 1 && share.part == 0 && column == 0 && threadIdx.x == 0)
-      c.header[1 + share.order] = {tile.seq, tile.row0, w, share.parts};
+    if (share.parts > 1) {
+      const int parts = min(share.parts, max(tiles_seen(c, tile.range, tile.length, tile.row0).count, 1));  // of these rows
+      if (share.part == 0 && column == 0 && threadIdx.x == 0)
+        c.header[1 + share.order] = {tile.seq, tile.row0, share.plane, parts > 1 ? parts : 0};
+      if (share.part >= parts) return;
+      share.parts = parts;
+    }
   } else if (!find_tile(c, c.slots - 1 - w, tile)) {  // late rows, the long ones, first
     return;
   }
-  float* plane = c.planes + ((int64_t)w * c.kv_heads + column) * (PROMPT_ROWS * (D + 2));
+  float* plane = c.planes + ((int64_t)(share.plane + share.part) * c.kv_heads + column) * (PROMPT_ROWS * (D + 2));
   prompt_tile<BF, D>(c, tile, column, share.part, share.parts, plane, c.s.table + (int64_t)tile.seq * c.s.width, lds);
 }
 
@@ -499,6 +522,7 @@ __global__ __launch_bounds__(256) void cache_prompt_join(PromptCall c) {
   const int column = (int)(blockIdx.x % c.kv_heads), rest = (int)(blockIdx.x / c.kv_heads), order = rest / BLOCKS;
   if (order >= c.header[0].x) return;
   const int4 head = c.header[1 + order];
+  if (head.w == 0) return;  // too few keys after all
   const TokenRange range = token_range(c.s, head.x);
   const int r = rest % BLOCKS * ROWS + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
   const int row = head.y + r, j = row / c.group;
@@ -530,12 +554,13 @@ PromptPlan krn::prompt_plan(int64_t tokens, int64_t step, int64_t group, int64_t
   PromptPlan p{};
   p.slots = p.workgroups = step > 0 ? sequences * ((step * group + PROMPT_ROWS - 1) / PROMPT_ROWS)
                                     : tokens * group / PROMPT_ROWS + sequences;
-  const int64_t shares = PROMPT_CUS / kv_heads;
-  if (width * page / PROMPT_TILE <= PROMPT_CHUNK || p.slots >= shares) return p;
-  // parts: as many as shares where there are fewer rows than that, else one each; at least two of every row that has several
-  const int64_t header = (shares / 2 + 1) * 16, need = header + shares * kv_heads * PROMPT_ROWS * (d + 2) * 4;
+  // parts beyond the first of all tiles of rows, in each column: as many as run at once without them, or half of that
+  const int64_t at_once = PROMPT_CUS / kv_heads, tiles = width * page / PROMPT_TILE;
+  if (at_once == 0 || tiles <= PROMPT_CHUNK || (p.slots >= at_once && (tiles <= PROMPT_LONG || sequences > 256))) return p;
+  const int64_t header = (at_once + 1) * 16, need = header + 2 * at_once * kv_heads * PROMPT_ROWS * (d + 2) * 4;
   if (need > bytes) return p;
-  p.shares = p.workgroups = shares, p.joins = shares / 2, p.header_bytes = header, p.bytes = need;
+  p.shares = p.workgroups = at_once > p.slots + at_once / 2 ? at_once : p.slots + at_once / 2;
+  p.spare = p.joins = at_once, p.header_bytes = header, p.bytes = need;
   return p;
 }
 
@@ -548,7 +573,7 @@ static void launch(const PromptCall& c, const PromptPlan& p, hipStream_t stream)
 }
 
 void krn::launch_cache_prompt(bool bf, int d, PromptCall c, const PromptPlan& p, void* workspace, hipStream_t stream) {
-  c.slots = (int)p.slots, c.shares = (uint32_t)p.shares;
+  c.slots = (int)p.slots, c.shares = (uint32_t)p.shares, c.spare = (uint32_t)p.spare;
   c.header = (int4*)workspace, c.planes = (float*)((char*)workspace + p.header_bytes);
   if (bf) d == 128 ? launch<true, 128>(c, p, stream) : launch<true, 64>(c, p, stream);
   else d == 128 ? launch<false, 128>(c, p, stream) : launch<false, 64>(c, p, stream);

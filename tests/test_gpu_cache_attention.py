@@ -315,6 +315,29 @@ def test_more_rows_than_run_at_once_are_those_of_each_sequence_alone(device, pac
         np.testing.assert_array_equal(got[rows], cache_attention(paged.tensor(q[rows].copy()), paged.cache, one).to_host())
 
 
+@pytest.mark.parametrize("prompt", [2000, 1300, 100])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_few_tokens_before_many_keys_beside_a_prompt(device, kind, prompt):
+    """The keys of some rows in parts, and rows that see fewer key tiles than their sequence has parts, beside whole ones."""
+    rng = np.random.default_rng(prompt)
+    counts, before = [1, prompt, 40, 0, 3, 30], [9000, 0, 8500, 7, 12000, 0]
+    lengths = [c + b for c, b in zip(counts, before)]
+    paged = Paged(device, rng, kind, lengths, kv_heads=8, d=64, page=32)
+    starts = [0, *np.cumsum(counts).tolist()]
+    q, exact = words(rng.standard_normal((starts[-1], 32, 64)), kind)
+    got = values(cache_attention(paged.tensor(q), paged.cache, paged.sequences(starts=starts)))
+    for i in (0, 2, 4, 5):
+        rows = slice(starts[i], starts[i + 1])
+        part = exact[rows]
+        one = Paged.__new__(Paged)
+        one.__dict__ = {**paged.__dict__, "table": paged.table[i : i + 1], "lengths": lengths[i : i + 1]}
+        assert_within(got[rows], *one.attention(part, [0, counts[i]]))
+    own = Sequences(device.to_device(np.array([prompt], np.int32)), device.to_device(paged.table[1:2, : -(-prompt // 32)].copy()),
+                    starts=device.to_device(np.array([0, prompt], np.int32)))
+    alone = values(cache_attention(paged.tensor(q[starts[1] : starts[2]].copy()), paged.cache, own))
+    np.testing.assert_array_equal(got[starts[1] : starts[2]], alone)
+
+
 def test_nothing_to_attend(device):
     paged = Paged(device, np.random.default_rng(1), "bf16", [], kv_heads=1, d=64)
     empty = device.empty(BF16, 0, 3, 64)
