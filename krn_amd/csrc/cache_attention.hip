@@ -67,7 +67,7 @@ extern "C" int krn_cache_attention(int kind, const void* q, const void* keys, co
   const int group = (int)(heads / kv_heads), span = window > 0x7fffffff ? 0 : (int)window;
   if (!starts && step * group <= TOKEN_ROWS) {
     const TokenPlan p = plan_of(tokens, heads, kv_heads, d, page, sequences, width, workspace ? workspace_bytes : 0);
-    if (p.workgroups * p.columns >= (int64_t)1 << 24) {
+    if (p.workgroups * kv_heads >= (int64_t)1 << 24) {
       krn_set_error("cache_attention: %lld sequences of %lld key heads", (long long)sequences, (long long)kv_heads);
       return -1;
     }

@@ -88,7 +88,9 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 
 // Attention of new tokens, a few of every sequence (cache_token.hip)
 constexpr int TOKEN_WAVES = 4;
-constexpr int TOKEN_ROWS = 64;     // rows of a key head, at most; more are a prompt's
+// Rows of a key head, at most; more are a prompt's. (64 sequences of 4000 keys, 64 heads on 8, d = 128: with one token each, 8 rows, 173 us
+// here; with 4, 32 rows, 207 here and 189 there; with 8, 64 rows in two more blocks, 270 and 193, but one sequence 20 and 24.)
+constexpr int TOKEN_ROWS = 32;
 // Parts that the keys of all sequences and columns are shared out to: two for each workgroup that runs at once. (64 sequences of
 // 4096 keys on average, d = 128: 512 parts 179 us, 1024 173, 2048 176; of 4096 each 164, 170, 175; 2 of 131000 103, 99, 102.)
 constexpr int TOKEN_PARTS = 1024;
@@ -97,8 +99,9 @@ constexpr int TOKEN_CHUNK = 4;
 // Tables of no more tiles a sequence keep each in one workgroup, which saves the joining launch (8 key heads, d = 128, one launch
 // and two: 300 keys 5.8 and 8.5 us, 256 sequences of 100 26.3 and 37.4, 16 of 200 8.7 and 10.5; 1000 keys 9.4 and 8.7)
 constexpr int TOKEN_WHOLE = 24;
-constexpr int TOKEN_SPLIT = 2048;  // sequences; more keep the keys of each in one workgroup
-constexpr int TOKEN_TILES = 1 << 20;  // of a sequence, as far as shares go by them: the sum of all stays below 2^32
+constexpr int TOKEN_SPLIT = 8192;  // sequences; more keep the keys of each in one workgroup
+constexpr int TOKEN_HELD = 4;      // sequences a lane counts
+constexpr int TOKEN_TILES = 1 << 18;  // of a sequence, as far as shares go by them: the sum of all stays below 2^32
 static_assert(TOKEN_PARTS + TOKEN_SPLIT < 1 << 16, "parts are counted in 16 bits");
 
 struct TokenCall {
@@ -108,16 +111,17 @@ struct TokenCall {
   SequencesView s;
   int heads, group, window;  // group: query heads of a key head
   float scale;               // of the scores, times log2(e)
-  int rows, row_groups, kept, columns, split;  // of TokenPlan
-  uint32_t shares;  // the parts of a column, with all sequences in one row
+  int rows, split;  // of TokenPlan
+  uint32_t shares;  // the parts of a key head, with all sequences in one row
   int4* header;     // the number of sequences in several parts, then of each (sequence, first workgroup, parts, -)
-  float* planes;    // of a workgroup and column: `kept` rows of sums, then their maxima and sums of weights
+  int4* map;        // of a workgroup (sequence or -1, part, parts, order of a sequence in several), if counted before
+  float* planes;    // of a workgroup and key head: `rows` rows of sums, then their maxima and sums of weights
 };
 
-// rows: of a key head; blocks: of sixteen rows that a workgroup takes; kept: its rows; columns: key heads times groups of rows
+// rows: of a key head
 struct TokenPlan {
-  int64_t rows, blocks, row_groups, kept, columns, shares, workgroups, joins, header_bytes, bytes;
-  bool split;
+  int64_t rows, shares, workgroups, joins, header_bytes, map_bytes, bytes;
+  bool split, mapped;
 };
 TokenPlan token_plan(int64_t step, int64_t group, int64_t kv_heads, int64_t d, int64_t page, int64_t sequences, int64_t width);
 void launch_cache_tokens(bool bf, int d, TokenCall c, const TokenPlan& p, void* workspace, hipStream_t stream);

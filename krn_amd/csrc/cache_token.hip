@@ -2,10 +2,10 @@
 // are multiplied with the head's keys and values, which are read once. What bounds it is that stream, so the keys of a
 // sequence are shared out over workgroups and joined by a second kernel.
 //
-// Shares. A tile is 32 keys. With T tiles in all sequences and C columns (key heads times groups of rows), a part has
-// at most chunk = max(TOKEN_CHUNK, T C / TOKEN_PARTS) tiles, and sequence i is ceil(tiles_i / chunk) parts of equal size:
-// long and short sequences together keep every CU busy to the end. Only the device knows the lengths, so each wave
-// counts the parts before its own.
+// Shares. A tile is 32 keys. With T tiles in all sequences and C key heads, a part has at most
+// chunk = max(TOKEN_CHUNK, T C / TOKEN_PARTS) tiles, and sequence i is ceil(tiles_i / chunk) parts of equal size: long and
+// short sequences together keep every CU busy to the end. Only the device knows the lengths, so each wave counts the parts
+// before its own or, with many sequences, a workgroup does for all (2000 sequences, one of 60000 keys and the others of 100: 259 us, by each wave 866).
 //
 // A wave computes S^T = K Q^T and O^T += V^T P^T with 16x16x32 MFMAs on its own tiles. A lane then holds one query row
 // (lane & 15) and eight keys of a tile: keys 4 g + r and 16 + 4 g + r, g = lane / 16, which are also the eight that it gives
@@ -120,34 +120,44 @@ struct Share {
   int seq, part, parts, order;
 };
 
-// Every wave counts for itself, a lane for ceil(n / 64) sequences in a row, so that no barrier is needed.
+__device__ __forceinline__ uint32_t weight_of(const TokenCall& c, int i) {
+  return (uint32_t)min(tiles_of(c, sequence_length(c.s, i)).count, TOKEN_TILES);
+}
+__device__ __forceinline__ uint32_t chunk_of(const TokenCall& c, uint32_t tiles) {
+  return max((uint32_t)TOKEN_CHUNK, (tiles + c.shares - 1) / c.shares);
+}
+__device__ __forceinline__ uint32_t parts_of(uint32_t weight, uint32_t chunk) { return max(1u, (weight + chunk - 1) / chunk); }
+// parts in the low half, sequences of several in the high one
+__device__ __forceinline__ uint32_t packed(uint32_t parts) { return parts + (parts > 1 ? 0x10000u : 0u); }
+
+// Every wave counts for itself, a lane for up to TOKEN_HELD sequences in a row, so that no barrier is needed. More
+// sequences are counted by a launch before this one.
 __device__ __forceinline__ bool find_share(const TokenCall& c, int w, bool writes, Share& share) {
   if (!c.split) {
     share = {w, 0, 1, 0};
     return true;
   }
-  constexpr int HELD = 4;  // sequences a lane keeps in registers
+  if (c.map) {
+    const int4 at = c.map[w];
+    share = {__builtin_amdgcn_readfirstlane(at.x), __builtin_amdgcn_readfirstlane(at.y), __builtin_amdgcn_readfirstlane(at.z),
+             __builtin_amdgcn_readfirstlane(at.w)};
+    return share.seq >= 0;
+  }
   const int lane = threadIdx.x & 63, per = (c.s.n + 63) / 64, first = lane * per, mine = max(0, min(per, c.s.n - first));
-  const auto weight_of = [&](int i) { return (uint32_t)min(tiles_of(c, sequence_length(c.s, i)).count, TOKEN_TILES); };
-  uint32_t held[HELD], tiles = 0;
+  uint32_t held[TOKEN_HELD], tiles = 0;
 #pragma unroll
-  for (int k = 0; k < HELD; ++k) {
-    held[k] = k < mine ? weight_of(first + k) : 0;
+  for (int k = 0; k < TOKEN_HELD; ++k) {
+    held[k] = k < mine ? weight_of(c, first + k) : 0;
     tiles += held[k];
   }
-  for (int k = HELD; k < mine; ++k) tiles += weight_of(first + k);
   tiles = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(tiles), 63);
-  const uint32_t chunk = max((uint32_t)TOKEN_CHUNK, (tiles + c.shares - 1) / c.shares);
-  // parts in the low half, sequences of several in the high one
-  const auto parts_of = [&](uint32_t weight) { return max(1u, (weight + chunk - 1) / chunk); };
-  const auto packed = [&](uint32_t parts) { return parts + (parts > 1 ? 0x10000u : 0u); };
+  const uint32_t chunk = chunk_of(c, tiles);
   uint32_t count = 0;
 #pragma unroll
-  for (int k = 0; k < HELD; ++k) {
-    held[k] = k < mine ? parts_of(held[k]) : 0;
+  for (int k = 0; k < TOKEN_HELD; ++k) {
+    held[k] = k < mine ? parts_of(held[k], chunk) : 0;
     count += packed(held[k]);
   }
-  for (int k = HELD; k < mine; ++k) count += packed(parts_of(weight_of(first + k)));
   const uint32_t upto = wave_scan(count), all = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
   if (writes && w == 0 && threadIdx.x == 0) c.header[0] = {(int)(all >> 16), 0, 0, 0};
   uint32_t before = upto - count;
@@ -155,7 +165,7 @@ __device__ __forceinline__ bool find_share(const TokenCall& c, int w, bool write
   if (owner == 0) return false;
   int seq = first, parts = 1;
   for (int k = 0; k < mine; ++k) {  // in the owner's lane: its sequence
-    parts = k < HELD ? (int)(k == 0 ? held[0] : k == 1 ? held[1] : k == 2 ? held[2] : held[3]) : (int)parts_of(weight_of(first + k));
+    parts = (int)(k == 0 ? held[0] : k == 1 ? held[1] : k == 2 ? held[2] : held[3]);
     if (w < (int)(before & 0xffff) + parts) {
       seq = first + k;
       break;
@@ -169,22 +179,56 @@ __device__ __forceinline__ bool find_share(const TokenCall& c, int w, bool write
   return true;
 }
 
+// The same for many sequences, once: the share of every workgroup of a column, a thread for `per` sequences in a row
+constexpr int MAP_THREADS = 1024;
+__global__ __launch_bounds__(MAP_THREADS) void cache_shares(TokenCall c, int workgroups) {
+  __shared__ uint32_t sums[2][MAP_THREADS / 64];
+  const int t = threadIdx.x, lane = t & 63, per = (c.s.n + MAP_THREADS - 1) / MAP_THREADS, first = t * per;
+  const int mine = max(0, min(per, c.s.n - first));
+  // the sum up to this thread, and of all
+  const auto scan = [&](uint32_t x, uint32_t* wave, uint32_t& all) {
+    const uint32_t upto = wave_scan(x);
+    if (lane == 63) wave[t / 64] = upto;
+    __syncthreads();
+    uint32_t before = 0;
+    all = 0;
+    for (int i = 0; i < MAP_THREADS / 64; ++i) {
+      before += i < t / 64 ? wave[i] : 0;
+      all += wave[i];
+    }
+    return before + upto;
+  };
+  uint32_t tiles = 0, all;
+  for (int k = 0; k < mine; ++k) tiles += weight_of(c, first + k);
+  scan(tiles, sums[0], all);
+  const uint32_t chunk = chunk_of(c, all);
+  uint32_t count = 0;
+  for (int k = 0; k < mine; ++k) count += packed(parts_of(weight_of(c, first + k), chunk));
+  uint32_t before = scan(count, sums[1], all) - count;
+  for (int k = 0; k < mine; ++k) {
+    const int parts = (int)parts_of(weight_of(c, first + k), chunk), from = (int)(before & 0xffff), order = (int)(before >> 16);
+    for (int p = 0; p < parts && from + p < workgroups; ++p) c.map[from + p] = {first + k, p, parts, order};
+    before += packed((uint32_t)parts);
+  }
+  for (int w = (int)(all & 0xffff) + t; w < workgroups; w += MAP_THREADS) c.map[w] = {-1, 0, 0, 0};
+  if (t == 0) c.header[0] = {(int)(all >> 16), 0, 0, 0};
+}
+
 template <bool BF, int D, int NB>
-__global__ __launch_bounds__(64 * TOKEN_WAVES, NB < 4 ? 2 : 1) void cache_tokens(TokenCall c) {
-  constexpr int RB = D * 2, DCH = D / 8, HALF = 16 * RB, TILE = 2 * HALF, LOADS = HALF / 1024, ROWS = 16 * NB;
+__global__ __launch_bounds__(64 * TOKEN_WAVES, 2) void cache_tokens(TokenCall c) {
+  constexpr int RB = D * 2, DCH = D / 8, HALF = 16 * RB, TILE = 2 * HALF, LOADS = HALF / 1024;
   constexpr int OLD = D + 4;  // floats per row of a wave's O in LDS
   static_assert(16 * OLD * 4 <= 2 * TILE, "a wave's rows fit its buffers");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[TOKEN_WAVES * 2 * TILE];
   __shared__ float stat[2][TOKEN_WAVES][16];
-  const int w = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / c.columns)), column = (int)blockIdx.x - w * c.columns;
+  const int w = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / c.cache.kv_heads)), kv = (int)blockIdx.x - w * c.cache.kv_heads;
   Share share;
-  if (!find_share(c, w, column == 0, share)) return;
+  if (!find_share(c, w, kv == 0, share)) return;
   const int seq = share.seq, part = share.part, parts = share.parts;
   const int t = threadIdx.x, lane = t & 63, g = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  if (parts > 1 && part == 0 && column == 0 && t == 0) c.header[1 + share.order] = {seq, w, parts, 0};
+  if (parts > 1 && part == 0 && kv == 0 && t == 0) c.header[1 + share.order] = {seq, w, parts, 0};
 
-  const int kv = __builtin_amdgcn_readfirstlane(column / c.row_groups), row0 = (column - kv * c.row_groups) * ROWS, rows = min(ROWS, c.rows - row0);
   const int length = __builtin_amdgcn_readfirstlane(sequence_length(c.s, seq)), end = held_keys(c.s, length, c.cache.page_shift);
   const TileRange range = tiles_of(c, length);
   // the part's tiles and this wave's (below 2^26), in scalar registers, where a division leaves none
@@ -197,7 +241,7 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES, NB < 4 ? 2 : 1) void cache_tokens
   int limit[NB], low[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    const int r = row0 + b * 16 + col, j = r / c.group;
+    const int r = b * 16 + col, j = r / c.group;
     const bool real = r < c.rows;
     const uint16_t* q = c.q + (((int64_t)seq * c.s.step + j) * c.heads + kv * c.group + (r - j * c.group)) * D;
 #pragma unroll
@@ -368,17 +412,17 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES, NB < 4 ? 2 : 1) void cache_tokens
 
   // the waves' rows meet in LDS, sixteen at a time: a lane has columns i * 16 + 4 g to + 3 of its row
   float* mine = reinterpret_cast<float*>(kbuf);
-  float* plane = c.planes + ((int64_t)w * c.columns + column) * c.kept * (D + 4);
+  float* plane = c.planes + ((int64_t)w * c.cache.kv_heads + kv) * c.rows * (D + 4);
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    if (b * 16 >= rows) break;
+    if (b * 16 >= c.rows) break;
     const float sum = row_sum(total[b]);
     __syncthreads();  // every wave is done with its tiles, or with the rows before
     if (g == 0) stat[0][wave][col] = m[b], stat[1][wave][col] = sum;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(mine + col * OLD + i * 16 + g * 4) = acc[b][i];
     __syncthreads();
-    for (int at = t; at < min(16, rows - b * 16) * (D / 4); at += 64 * TOKEN_WAVES) {
+    for (int at = t; at < min(16, c.rows - b * 16) * (D / 4); at += 64 * TOKEN_WAVES) {
       const int row = at / (D / 4), d = at % (D / 4) * 4;
       float top = stat[0][0][row];
 #pragma unroll
@@ -395,9 +439,9 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES, NB < 4 ? 2 : 1) void cache_tokens
       if (parts > 1) {  // unnormalised rows, then their maxima and sums
         const int r = b * 16 + row;
         *reinterpret_cast<f32x4*>(plane + r * D + d) = o;
-        if (d == 0) plane[c.kept * D + r * 2] = top, plane[c.kept * D + r * 2 + 1] = all;
+        if (d == 0) plane[c.rows * D + r * 2] = top, plane[c.rows * D + r * 2 + 1] = all;
       } else {
-        const int r = row0 + b * 16 + row, j = r / c.group;
+        const int r = b * 16 + row, j = r / c.group;
         const float inv = all == 0.0f ? 0.0f : 1.0f / all;  // no key: zeros
         const u32x2 y = {Narrow<BF>::pack(o[0] * inv, o[1] * inv), Narrow<BF>::pack(o[2] * inv, o[3] * inv)};
         *reinterpret_cast<u32x2*>(c.o + (((int64_t)seq * c.s.step + j) * c.heads + kv * c.group + (r - j * c.group)) * D + d) = y;
@@ -413,20 +457,18 @@ __global__ __launch_bounds__(JOIN_THREADS) void cache_join(TokenCall c) {
   constexpr int LANES = JOIN_THREADS / (D / 4);
   __shared__ f32x4 sums[LANES][D / 4];
   __shared__ float stat[2][LANES];
-  const int rest = (int)(blockIdx.x / c.columns), column = (int)(blockIdx.x % c.columns), order = rest / c.kept, r = rest % c.kept;
+  const int rest = (int)(blockIdx.x / c.cache.kv_heads), kv = (int)(blockIdx.x % c.cache.kv_heads), order = rest / c.rows, r = rest % c.rows;
   if (order >= c.header[0].x) return;
   const int4 head = c.header[1 + order];
-  const int kv = column / c.row_groups, row = column % c.row_groups * c.kept + r;
-  if (row >= c.rows) return;
   const int t = threadIdx.x, side = t / (D / 4), d = t % (D / 4) * 4;
-  const int64_t stride = (int64_t)c.columns * c.kept * (D + 4);
-  const float* plane = c.planes + head.y * stride + (int64_t)column * c.kept * (D + 4);
+  const int64_t stride = (int64_t)c.cache.kv_heads * c.rows * (D + 4);
+  const float* plane = c.planes + head.y * stride + (int64_t)kv * c.rows * (D + 4);
   float m = -INFINITY, total = 0.0f;
   f32x4 o = f32x4{};
 #pragma unroll 4
   for (int p = side; p < head.z; p += LANES) {
     const float* at = plane + p * stride;
-    const float top = at[c.kept * D + r * 2], sum = at[c.kept * D + r * 2 + 1], next = fmaxf(m, top);
+    const float top = at[c.rows * D + r * 2], sum = at[c.rows * D + r * 2 + 1], next = fmaxf(m, top);
     const float to_base = next == -INFINITY ? 0.0f : next;
     const float f = __builtin_amdgcn_exp2f(m - to_base), h = __builtin_amdgcn_exp2f(top - to_base);
     total = total * f + sum * h;
@@ -450,9 +492,9 @@ __global__ __launch_bounds__(JOIN_THREADS) void cache_join(TokenCall c) {
     o += f * sums[x][d / 4];
   }
   const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-  const int j = row / c.group;
+  const int j = r / c.group;
   const u32x2 y = {Narrow<BF>::pack(o[0] * inv, o[1] * inv), Narrow<BF>::pack(o[2] * inv, o[3] * inv)};
-  *reinterpret_cast<u32x2*>(c.o + (((int64_t)head.x * c.s.step + j) * c.heads + kv * c.group + (row - j * c.group)) * D + d) = y;
+  *reinterpret_cast<u32x2*>(c.o + (((int64_t)head.x * c.s.step + j) * c.heads + kv * c.group + (r - j * c.group)) * D + d) = y;
 }
 
 }  // namespace krn
@@ -462,38 +504,35 @@ using namespace krn;
 TokenPlan krn::token_plan(int64_t step, int64_t group, int64_t kv_heads, int64_t d, int64_t page, int64_t sequences, int64_t width) {
   TokenPlan p{};
   p.rows = step * group;
-  p.blocks = p.rows <= 16 ? 1 : p.rows <= 32 ? 2 : 4;
-  p.row_groups = (p.rows + 16 * p.blocks - 1) / (16 * p.blocks);
-  p.kept = p.rows < 16 * p.blocks ? p.rows : 16 * p.blocks;
-  p.columns = kv_heads * p.row_groups;
   const int64_t tiles = (width * page < 0x7fffffff ? width * page : 0x7fffffff) / 32 + 1;  // of a sequence, at most
-  // parts beyond the first of all sequences, in each column: no more than shares, nor than parts have tiles
-  p.shares = TOKEN_PARTS / p.columns;
+  // parts beyond the first of all sequences, for each key head: no more than shares, nor than parts have tiles
+  p.shares = TOKEN_PARTS / kv_heads;
   int64_t extra = p.shares;
   if (sequences * ((tiles - 1) / TOKEN_CHUNK) < extra) extra = sequences * ((tiles - 1) / TOKEN_CHUNK);
   if (sequences > TOKEN_SPLIT || tiles - 1 <= TOKEN_WHOLE) extra = 0;
   p.workgroups = sequences + extra;
-  p.split = extra > 0;
+  p.split = extra > 0, p.mapped = p.split && sequences > 64 * TOKEN_HELD;
   p.joins = sequences < extra ? sequences : extra;
   p.header_bytes = p.split ? (p.joins + 1) * 16 : 0;
-  p.bytes = p.split ? p.header_bytes + p.workgroups * p.columns * p.kept * (d + 4) * 4 : 0;
+  p.map_bytes = p.mapped ? p.workgroups * 16 : 0;
+  p.bytes = p.split ? p.header_bytes + p.map_bytes + p.workgroups * kv_heads * p.rows * (d + 4) * 4 : 0;
   return p;
 }
 
 template <bool BF, int D>
 static void launch(const TokenCall& c, const TokenPlan& p, hipStream_t stream) {
-  const dim3 grid((unsigned)(p.workgroups * p.columns)), block(64 * TOKEN_WAVES);
-  if (p.blocks == 1) hipLaunchKernelGGL((cache_tokens<BF, D, 1>), grid, block, 0, stream, c);
-  else if (p.blocks == 2) hipLaunchKernelGGL((cache_tokens<BF, D, 2>), grid, block, 0, stream, c);
-  else hipLaunchKernelGGL((cache_tokens<BF, D, 4>), grid, block, 0, stream, c);
+  const dim3 grid((unsigned)(p.workgroups * c.cache.kv_heads)), block(64 * TOKEN_WAVES);
+  if (c.map) hipLaunchKernelGGL(cache_shares, dim3(1), dim3(MAP_THREADS), 0, stream, c, (int)p.workgroups);
+  if (p.rows <= 16) hipLaunchKernelGGL((cache_tokens<BF, D, 1>), grid, block, 0, stream, c);
+  else hipLaunchKernelGGL((cache_tokens<BF, D, 2>), grid, block, 0, stream, c);
   if (c.split)
-    hipLaunchKernelGGL((cache_join<BF, D>), dim3((unsigned)(p.joins * p.kept * p.columns)), dim3(JOIN_THREADS), 0, stream, c);
+    hipLaunchKernelGGL((cache_join<BF, D>), dim3((unsigned)(p.joins * p.rows * c.cache.kv_heads)), dim3(JOIN_THREADS), 0, stream, c);
 }
 
 void krn::launch_cache_tokens(bool bf, int d, TokenCall c, const TokenPlan& p, void* workspace, hipStream_t stream) {
-  c.rows = (int)p.rows, c.row_groups = (int)p.row_groups, c.kept = (int)p.kept, c.columns = (int)p.columns, c.split = p.split;
-  c.shares = (uint32_t)p.shares;
-  c.header = (int4*)workspace, c.planes = (float*)((char*)workspace + p.header_bytes);
+  c.rows = (int)p.rows, c.split = p.split, c.shares = (uint32_t)p.shares;
+  c.header = (int4*)workspace, c.map = p.mapped ? (int4*)((char*)workspace + p.header_bytes) : nullptr;
+  c.planes = (float*)((char*)workspace + p.header_bytes + p.map_bytes);
   if (bf) d == 128 ? launch<true, 128>(c, p, stream) : launch<true, 64>(c, p, stream);
   else d == 128 ? launch<false, 128>(c, p, stream) : launch<false, 64>(c, p, stream);
 }

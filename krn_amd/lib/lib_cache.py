@@ -168,7 +168,7 @@ def cache_attention(q, cache: KvCache, sequences: Sequences, *, scale: float | N
     heads share a key head; scale is 1 / sqrt(d) unless given. A token without keys gets zeros. Keys and values that a token
     does not see have no part in its result, NaN and infinities included; pages wholly before the windows of all new tokens
     may be another sequence's. Scores, maxima and sums are float32; softmax weights are rounded to 16 bits before they multiply
-    values, to two 16-bit parts where sequences have up to 64 rows, new tokens times query heads of a key head. `out` may be q
+    values, to two 16-bit parts where sequences have up to 32 rows, new tokens times query heads of a key head. `out` may be q
     itself and shares no other memory. Sequences of as many new tokens each, a few, are faster without `starts`."""
     _checked(cache, sequences)
     tensor(q, "q", 3, (cache.dtype,))

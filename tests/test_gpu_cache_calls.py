@@ -210,6 +210,18 @@ def test_without_a_workspace_the_keys_stay_in_one_workgroup(device):
             assert_within(values(o), *paged.attention(exact, starts or [0, 1, 2]))
 
 
+@pytest.mark.parametrize("n", [255, 256, 257, 1030])
+@pytest.mark.parametrize("new", [1, 2])
+def test_many_sequences_some_of_them_long(device, n, new):
+    rng = np.random.default_rng(n)
+    lengths = rng.integers(0, 60, n).tolist()
+    lengths[0], lengths[n // 2], lengths[n - 1] = 3000, 1000, 5000
+    paged = Paged(device, rng, "bf16", lengths, kv_heads=2, d=64)
+    q, exact = words(rng.standard_normal((n * new, 4, 64)), "bf16")
+    got = values(cache_attention(paged.tensor(q), paged.cache, paged.sequences(new=new)))
+    assert_within(got, *paged.attention(exact, list(range(0, n * new + 1, new))))
+
+
 def test_many_sequences(device):
     """More sequences than are shared out or searched in one look, of one token and of a few."""
     rng = np.random.default_rng(9)
