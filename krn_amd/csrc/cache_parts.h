@@ -134,7 +134,7 @@ constexpr int PROMPT_ROWS = 128;  // of a workgroup: tokens times query heads of
 constexpr int PROMPT_CHUNK = 16;
 // Tiles of a table, beyond which rows are shared out where they fill the chip as well: a single token before 65000 keys, packed
 // with a prompt of 2000 tokens, would run on alone (891 us, shared out 131). Counting parts and the joining launch cost 60
-// prompts of 150 tokens with such a table 53.6 and 59.1.
+// prompts of 150 tokens with such a table 53.0 and 56.7.
 constexpr int PROMPT_LONG = 128;
 constexpr int PROMPT_CUS = 512;  // workgroups that run at once
 

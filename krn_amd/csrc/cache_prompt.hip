@@ -515,34 +515,37 @@ __global__ __launch_bounds__(64 * PROMPT_WAVES, 2) void cache_prompt(PromptCall 
   prompt_tile<BF, D>(c, tile, column, share.part, share.parts, plane, c.s.table + (int64_t)tile.seq * c.s.width, lds);
 }
 
-// Rows in several parts: four columns of a row a thread, the parts one after the other
+// Rows in several parts: four columns of a row a thread, the parts one after the other. No more workgroups than run at once: most
+// calls have far fewer rows to join than they may have.
+constexpr int JOIN_GROUPS = 2048;
 template <bool BF, int D>
 __global__ __launch_bounds__(256) void cache_prompt_join(PromptCall c) {
   constexpr int ROWS = 256 / (D / 4), BLOCKS = PROMPT_ROWS / ROWS;  // of a workgroup, of a tile of rows
-  const int column = (int)(blockIdx.x % c.kv_heads), rest = (int)(blockIdx.x / c.kv_heads), order = rest / BLOCKS;
-  if (order >= c.header[0].x) return;
-  const int4 head = c.header[1 + order];
-  if (head.w == 0) return;  // too few keys after all
-  const TokenRange range = token_range(c.s, head.x);
-  const int r = rest % BLOCKS * ROWS + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
-  const int row = head.y + r, j = row / c.group;
-  if (j >= range.count) return;
-  const int64_t stride = (int64_t)c.kv_heads * (PROMPT_ROWS * (D + 2));
-  const float* plane = c.planes + head.z * stride + (int64_t)column * (PROMPT_ROWS * (D + 2));
-  float m = -INFINITY, all = 0.0f;
-  f32x4 o = f32x4{};
+  const int items = c.header[0].x * BLOCKS * c.kv_heads;
+  for (int item = (int)blockIdx.x; item < items; item += (int)gridDim.x) {
+    const int column = item % c.kv_heads, rest = item / c.kv_heads;
+    const int4 head = c.header[1 + rest / BLOCKS];
+    const TokenRange range = token_range(c.s, head.x);
+    const int r = rest % BLOCKS * ROWS + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+    const int row = head.y + r, j = row / c.group;
+    if (head.w == 0 || j >= range.count) continue;  // too few keys after all, or no row
+    const int64_t stride = (int64_t)c.kv_heads * (PROMPT_ROWS * (D + 2));
+    const float* plane = c.planes + head.z * stride + (int64_t)column * (PROMPT_ROWS * (D + 2));
+    float m = -INFINITY, all = 0.0f;
+    f32x4 o = f32x4{};
 #pragma unroll 4
-  for (int p = 0; p < head.w; ++p) {
-    const float* at = plane + p * stride;
-    const float top = at[PROMPT_ROWS * D + r * 2], next = fmaxf(m, top), to_base = next == -INFINITY ? 0.0f : next;
-    const float f = __builtin_amdgcn_exp2f(m - to_base), h = __builtin_amdgcn_exp2f(top - to_base);
-    all = all * f + at[PROMPT_ROWS * D + r * 2 + 1] * h;
-    o = o * f + h * *reinterpret_cast<const f32x4*>(at + r * D + d);
-    m = next;
+    for (int p = 0; p < head.w; ++p) {
+      const float* at = plane + p * stride;
+      const float top = at[PROMPT_ROWS * D + r * 2], next = fmaxf(m, top), to_base = next == -INFINITY ? 0.0f : next;
+      const float f = __builtin_amdgcn_exp2f(m - to_base), h = __builtin_amdgcn_exp2f(top - to_base);
+      all = all * f + at[PROMPT_ROWS * D + r * 2 + 1] * h;
+      o = o * f + h * *reinterpret_cast<const f32x4*>(at + r * D + d);
+      m = next;
+    }
+    const float inv = all == 0.0f ? 0.0f : 1.0f / all;  // no key: zeros
+    const u32x2 y = {Half<BF>::pack(o[0] * inv, o[1] * inv), Half<BF>::pack(o[2] * inv, o[3] * inv)};
+    *reinterpret_cast<u32x2*>(c.o + ((int64_t)(range.first + j) * c.heads + column * c.group + (row - j * c.group)) * D + d) = y;
   }
-  const float inv = all == 0.0f ? 0.0f : 1.0f / all;  // no key: zeros
-  const u32x2 y = {Half<BF>::pack(o[0] * inv, o[1] * inv), Half<BF>::pack(o[2] * inv, o[3] * inv)};
-  *reinterpret_cast<u32x2*>(c.o + ((int64_t)(range.first + j) * c.heads + column * c.group + (row - j * c.group)) * D + d) = y;
 }
 
 }  // namespace krn
@@ -567,9 +570,9 @@ PromptPlan krn::prompt_plan(int64_t tokens, int64_t step, int64_t group, int64_t
 template <bool BF, int D>
 static void launch(const PromptCall& c, const PromptPlan& p, hipStream_t stream) {
   hipLaunchKernelGGL((cache_prompt<BF, D>), dim3((unsigned)(p.workgroups * c.kv_heads)), dim3(64 * PROMPT_WAVES), 0, stream, c);
+  const int64_t items = p.joins * (PROMPT_ROWS * (D / 4) / 256) * c.kv_heads;
   if (p.shares)
-    hipLaunchKernelGGL((cache_prompt_join<BF, D>), dim3((unsigned)(p.joins * (PROMPT_ROWS * (D / 4) / 256) * c.kv_heads)),
-                       dim3(256), 0, stream, c);
+    hipLaunchKernelGGL((cache_prompt_join<BF, D>), dim3((unsigned)(items < JOIN_GROUPS ? items : JOIN_GROUPS)), dim3(256), 0, stream, c);
 }
 
 void krn::launch_cache_prompt(bool bf, int d, PromptCall c, const PromptPlan& p, void* workspace, hipStream_t stream) {
