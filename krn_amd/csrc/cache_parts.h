@@ -100,7 +100,9 @@ constexpr int TOKEN_CHUNK = 4;
 // and two: 300 keys 5.8 and 8.5 us, 256 sequences of 100 26.3 and 37.4, 16 of 200 8.7 and 10.5; 1000 keys 9.4 and 8.7)
 constexpr int TOKEN_WHOLE = 24;
 constexpr int TOKEN_SPLIT = 8192;  // sequences; more keep the keys of each in one workgroup
-constexpr int TOKEN_HELD = 4;      // sequences a lane counts
+// Sequences that a lane counts; beyond 64 times as many a launch counts them first (128 sequences of 100 keys 19.2 us, 19.8 with it,
+// 256 36.2 and 31)
+constexpr int TOKEN_HELD = 2;
 constexpr int TOKEN_TILES = 1 << 18;  // of a sequence, as far as shares go by them: the sum of all stays below 2^32
 static_assert(TOKEN_PARTS + TOKEN_SPLIT < 1 << 16, "parts are counted in 16 bits");
 

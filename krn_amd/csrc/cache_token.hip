@@ -5,7 +5,7 @@
 // Shares. A tile is 32 keys. With T tiles in all sequences and C key heads, a part has at most
 // chunk = max(TOKEN_CHUNK, T C / TOKEN_PARTS) tiles, and sequence i is ceil(tiles_i / chunk) parts of equal size: long and
 // short sequences together keep every CU busy to the end. Only the device knows the lengths, so each wave counts the parts
-// before its own or, with many sequences, a workgroup does for all (2000 sequences, one of 60000 keys and the others of 100:
+// before its own or, with more than 128 sequences, a workgroup does for all (2000 sequences, one of 60000 keys and the others of 100:
 // 259 us, by each wave 866).
 //
 // A wave computes S^T = K Q^T and O^T += V^T P^T with 16x16x32 MFMAs on its own tiles. A lane then holds one query row
@@ -165,13 +165,13 @@ __device__ __forceinline__ bool find_share(const TokenCall& c, int w, bool write
   const uint64_t owner = __builtin_amdgcn_ballot_w64((int)(before & 0xffff) <= w && w < (int)(upto & 0xffff));
   if (owner == 0) return false;
   int seq = first, parts = 1;
-  for (int k = 0; k < mine; ++k) {  // in the owner's lane: its sequence
-    parts = (int)(k == 0 ? held[0] : k == 1 ? held[1] : k == 2 ? held[2] : held[3]);
-    if (w < (int)(before & 0xffff) + parts) {
-      seq = first + k;
-      break;
-    }
-    before += packed((uint32_t)parts);
+  bool found = false;
+#pragma unroll
+  for (int k = 0; k < TOKEN_HELD; ++k) {  // in the owner's lane: its sequence
+    if (found || k >= mine) continue;
+    seq = first + k, parts = (int)held[k];
+    found = w < (int)(before & 0xffff) + parts;
+    if (!found) before += packed(held[k]);
   }
   const int from = __builtin_ctzll(owner);
   share.seq = __builtin_amdgcn_readlane(seq, from), share.parts = __builtin_amdgcn_readlane(parts, from);

@@ -210,7 +210,7 @@ def test_without_a_workspace_the_keys_stay_in_one_workgroup(device):
             assert_within(values(o), *paged.attention(exact, starts or [0, 1, 2]))
 
 
-@pytest.mark.parametrize("n", [255, 256, 257, 1030])
+@pytest.mark.parametrize("n", [63, 65, 127, 128, 129, 256, 1030])
 @pytest.mark.parametrize("new", [1, 2])
 def test_many_sequences_some_of_them_long(device, n, new):
     rng = np.random.default_rng(n)
