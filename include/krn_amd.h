@@ -184,9 +184,9 @@ int64_t krn_moe_workspace(int kind, int64_t tokens, int64_t hidden, int64_t inne
 /* A paged key-value cache: `keys` and `values` are each pages x kv_heads x page x d, of kind KRN_F16 or KRN_BF16, d 64 or 128,
  * page a power of two from 16 to 65536, 16-byte aligned. The sequences of a step: `lengths` (sequences) counts the keys of each,
  * those of its newest tokens included, and `table` (sequences x width, width * page below 2^31 - 255) numbers the pages that it
- * owns: key j of sequence i lies in row j % page of page table[i, j / page]. The step's tokens are packed; those of sequence i are starts[i] to
- * starts[i + 1] - 1 (`starts` has sequences + 1 entries and does not decrease) or, with starts NULL, `step` for every sequence
- * (tokens = step * sequences). Its last token has position lengths[i] - 1. All three arrays are int32 on the device and are read
+ * owns: key j of sequence i lies in row j % page of page table[i, j / page]. The step's tokens are packed; those of sequence i
+ * are starts[i] to starts[i + 1] - 1 (`starts` has sequences + 1 entries and does not decrease) or, with starts NULL, `step` for
+ * every sequence (tokens = step * sequences). Its last token has position lengths[i] - 1. All three arrays are int32 on the device and are read
  * when the kernels run. They are checked there: a token that no range holds belongs to no sequence and what would be written
  * for it stays as it was, keys beyond width pages are not there, a page number outside of the cache reads as zeros and is
  * not written. No counterpart in the reference, whose attention reads dense tensors.
@@ -205,10 +205,11 @@ int krn_rotary_append(int kind, const void* qkv, void* q, void* keys, void* valu
 /* o = softmax(scale q K^T) V, causal: a token at position p attends to its sequence's keys up to p, to the last `window` of them
  * if that is not 0. q and o are tokens x heads x d; heads / kv_heads query heads share a key head; scale > 0. A token without
  * keys gets zeros. Keys and values that a token does not see have no part in its result, NaN and infinities included; pages that
- * lie wholly before the windows of all new tokens may belong to other sequences. Weights are rounded to 16 bits before they multiply values, to two 16-bit parts without starts and with up to 32
- * rows (step * heads / kv_heads). o may be q itself and shares no other memory. A workspace of krn_cache_attention_workspace bytes (`packed`:
- * with starts; 16-byte aligned, no preparation, not touched by other work until this call's has run; calls on one stream may
- * share one) lets the keys of one token be split over workgroups; with less, or none, they stay in one. */
+ * lie wholly before the windows of all new tokens may belong to other sequences. Weights are rounded to 16 bits before they
+ * multiply values, to two 16-bit parts without starts and with up to 32 rows (step * heads / kv_heads). o may be q itself and
+ * shares no other memory. A workspace of krn_cache_attention_workspace bytes (`packed`: with starts; 16-byte aligned, no
+ * preparation, not touched by other work until this call's has run; calls on one stream may share one) lets the keys of one
+ * token be split over workgroups; with less, or none, they stay in one. */
 int krn_cache_attention(int kind, const void* q, const void* keys, const void* values, void* o, int64_t tokens, int64_t heads,
                         int64_t kv_heads, int64_t d, int64_t pages, int64_t page, const int* starts, int64_t step,
                         const int* lengths, const int* table, int64_t sequences, int64_t width, float scale, int64_t window,

@@ -88,8 +88,8 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 
 // Attention of new tokens, a few of every sequence (cache_token.hip)
 constexpr int TOKEN_WAVES = 4;
-// Rows of a key head, at most; more are a prompt's. (64 sequences of 4000 keys, 64 heads on 8, d = 128: with one token each, 8 rows, 173 us
-// here; with 4, 32 rows, 207 here and 189 there; with 8, 64 rows in two more blocks, 270 and 193, but one sequence 20 and 24.)
+// Rows of a key head, at most; more are a prompt's. (64 sequences of 4000 keys, d = 128, 8 key heads: 32 rows 207 us here
+// and 189 there, but one sequence 12 and 24; 64 rows, in two more blocks of sixteen, 270 and 193, one sequence 20 and 24.)
 constexpr int TOKEN_ROWS = 32;
 // Parts that the keys of all sequences and columns are shared out to: two for each workgroup that runs at once. (64 sequences of
 // 4096 keys on average, d = 128: 512 parts 179 us, 1024 173, 2048 176; of 4096 each 164, 170, 175; 2 of 131000 103, 99, 102.)
@@ -100,8 +100,8 @@ constexpr int TOKEN_CHUNK = 4;
 // and two: 300 keys 5.8 and 8.5 us, 256 sequences of 100 26.3 and 37.4, 16 of 200 8.7 and 10.5; 1000 keys 9.4 and 8.7)
 constexpr int TOKEN_WHOLE = 24;
 constexpr int TOKEN_SPLIT = 8192;  // sequences; more keep the keys of each in one workgroup
-// Sequences that a lane counts; beyond 64 times as many a launch counts them first (128 sequences of 100 keys 19.2 us, 19.8 with it,
-// 256 36.2 and 31)
+// Sequences that a lane counts; beyond 64 times as many a launch counts them first (128 sequences of 100 keys 19.2 us, 19.8
+// with it, 256 36.2 and 31)
 constexpr int TOKEN_HELD = 2;
 constexpr int TOKEN_TILES = 1 << 18;  // of a sequence, as far as shares go by them: the sum of all stays below 2^32
 static_assert(TOKEN_PARTS + TOKEN_SPLIT < 1 << 16, "parts are counted in 16 bits");
@@ -131,8 +131,8 @@ void launch_cache_tokens(bool bf, int d, TokenCall c, const TokenPlan& p, void* 
 // Attention of packed prompts (cache_prompt.hip)
 constexpr int PROMPT_ROWS = 128;  // of a workgroup: tokens times query heads of a key head
 
-// Tiles of 64 keys of a part, at least: a part costs 67 KB of sums written and read (128 tokens after 8000, 32 heads on 8: 35.0 us,
-// with 8 40.9, with 32 43.4)
+// Tiles of 64 keys of a part, at least: a part costs 67 KB of sums written and read (128 tokens after 8000, 32 heads on 8:
+// 32.5 us, with 8 36.6, with 32 41.9)
 constexpr int PROMPT_CHUNK = 16;
 // Tiles of a table, beyond which rows are shared out where they fill the chip as well: a single token before 65000 keys, packed
 // with a prompt of 2000 tokens, would run on alone (891 us, shared out 131). Counting parts and the joining launch cost 60

@@ -5,14 +5,15 @@
 // its four waves owns 32 rows and computes S^T = K Q^T and O^T += V^T P^T with 32x32x16 MFMAs: a lane holds one row
 // (lane & 31) and half of the keys (its partner is lane ^ 32), P stays in its lane.
 //
-// The matrix cores and the power that they draw bound it (16384 tokens, 32 heads of 128 on 8: 1.87 to 1.96 ms by the card, 1120
-// to 1180 TFLOP/s; a large library product reaches 1380). Two workgroups share a CU, two waves a SIMD. Each wave interleaves its
-// own work: scores of the next tile beside the weights of this one, then O += P V beside the exponents of the next, one MFMA
-// and a few other instructions at a time in the order written (left to the compiler, 2 % slower). The other workgroup covers
-// what comes before and after the loop: one workgroup of eight waves a CU reads keys half as often and has 0 to 2 % on that one prompt,
-// 5 on 512 tokens after 15900, but 12 prompts of 8192 tokens take 153 us in place of 144, 16 of 500 10.0 and 8.5, 1024 tokens 29.0
-// and 22.5. (Eight waves in two groups that take turns by barriers: 2.06 ms. Four of 64 rows halve the LDS reads, but need more
-// than 256 registers: 2.27 ms with the compiler's copies, 2.04 with accumulators that products alone touch.)
+// The matrix cores and the power that they draw bound it (16384 tokens, 32 heads of 128 on 8: 1.85 to 1.99 ms by the card,
+// 1105 to 1185 TFLOP/s; a large library product reaches 1380). Two workgroups share a CU, two waves a SIMD. Each wave
+// interleaves its own work: scores of the next tile beside the weights of this one, then O += P V beside the exponents of
+// the next, one MFMA and a few other instructions at a time in the order written (left to the compiler, 2 % slower). The
+// other workgroup covers what comes before and after the loop: one workgroup of eight waves a CU reads keys half as often
+// and has 0 to 2 % on that one prompt, 5 on 512 tokens after 15900, but 12 prompts of 8192 tokens take 153 us in place of
+// 144, 16 of 500 10.0 and 8.5, 1024 tokens 29.0 and 22.5. (Eight waves in two groups that take turns by barriers: 2.06 ms.
+// Four of 64 rows halve the LDS reads, but need more than 256 registers: 2.27 ms with the compiler's copies, 2.04 with
+// accumulators that products alone touch.)
 //
 // K and V come into rings of three and two tiles by direct loads, more than a tile ahead of their use; tiles past the end are
 // asked for with no bytes, which keeps the count of loads on their way the same. Sixteen keys, a wave's part of a tile, lie in
@@ -84,10 +85,11 @@ __device__ __forceinline__ KeyTiles tiles_seen(const PromptCall& c, const TokenR
   return {first, max(0, (max(end, 0) + PROMPT_TILE - 1) / PROMPT_TILE - first)};
 }
 
-// Rows before many keys are shared out: workgroup w of a column does part `part` of `parts` of a tile of rows. All tiles of rows of a
-// sequence have as many parts, so that nothing loops over them: with R of them of up to T key tiles each, ceil(T / chunk), and chunk
-// is the sum of all R T over `spare`, the workgroups that are there beyond one for each tile of rows. Every wave counts
-// for itself, a lane for ceil(n / 64) sequences in a row. What no chip does in a second stays whole, and the sums below 2^32.
+// Rows before many keys are shared out: workgroup w of a column does part `part` of `parts` of a tile of rows. All tiles of
+// rows of a sequence have as many parts, so that nothing loops over them: with R of them of up to T key tiles each, ceil(T
+// / chunk), and chunk is the sum of all R T over `spare`, the workgroups that are there beyond one for each tile of rows.
+// Every wave counts for itself, a lane for ceil(n / 64) sequences in a row. What no chip does in a second stays whole, and
+// the sums below 2^32.
 struct PromptPart {
   int part, parts, plane, order;  // plane: of the first part, among all planes; order: of the rows, among those in several parts
 };
@@ -188,7 +190,7 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
   // this lane's row, the keys that it sees, and those that all or some rows of the wave and the workgroup see
   const int row = tile.row0 + wave * 32 + r32, j = row / c.group;
   const bool real = j < tile.range.count;
-  const int limit = min(before + min(j, tile.range.count - 1) + 1, end), low = first_key(before + min(j, tile.range.count - 1), c.window);
+  const int position = before + min(j, tile.range.count - 1), limit = min(position + 1, end), low = first_key(position, c.window);
   const int all_limit = __builtin_amdgcn_readfirstlane(limit), all_low = __builtin_amdgcn_readlane(low, 31);
   // tiles within these bounds have keys that all rows of the workgroup see, or that lie past the end and are zeros
   const int last_token = min((tile.row0 + PROMPT_ROWS - 1) / c.group, tile.range.count - 1);

@@ -2,11 +2,11 @@
 // are multiplied with the head's keys and values, which are read once. What bounds it is that stream, so the keys of a
 // sequence are shared out over workgroups and joined by a second kernel.
 //
-// Shares. A tile is 32 keys. With T tiles in all sequences and C key heads, a part has at most
-// chunk = max(TOKEN_CHUNK, T C / TOKEN_PARTS) tiles, and sequence i is ceil(tiles_i / chunk) parts of equal size: long and
-// short sequences together keep every CU busy to the end. Only the device knows the lengths, so each wave counts the parts
-// before its own or, with more than 128 sequences, a workgroup does for all (2000 sequences, one of 60000 keys and the others of 100:
-// 259 us, by each wave 866).
+// Shares. A tile is 32 keys. With T tiles in all sequences and C key heads, a part has at most chunk = max(TOKEN_CHUNK, T C
+// / TOKEN_PARTS) tiles, and sequence i is ceil(tiles_i / chunk) parts of equal size: long and short sequences together keep
+// every CU busy to the end. Only the device knows the lengths, so each wave counts the parts before its own or, with more
+// than 128 sequences, a workgroup does for all (2000 sequences, one of 60000 keys and the others of 100: 259 us, by each
+// wave 866).
 //
 // A wave computes S^T = K Q^T and O^T += V^T P^T with 16x16x32 MFMAs on its own tiles. A lane then holds one query row
 // (lane & 15) and eight keys of a tile: keys 4 g + r and 16 + 4 g + r, g = lane / 16, which are also the eight that it gives
