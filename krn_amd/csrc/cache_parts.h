@@ -37,6 +37,12 @@ __device__ __forceinline__ int first_key(int position, int window) {
   return window ? (int)max((int64_t)0, (int64_t)position + 1 - window) : 0;
 }
 
+// Softmax weights are rounded to 16 bits before their products. In f16, whose last step is 2^-24, they are 2^7 times as large,
+// up to 2^15 with the margin of 2^8 by which a weight may exceed the first: what is below 2^-32 of the largest is lost (2^-25
+// without the factor, 0.4 % of a result of 131000 keys behind one large weight). The sums of weights have it too.
+template <bool BF>
+constexpr float LIFT = BF ? 0.0f : 7.0f;
+
 // Values that are not finite: a weight of zero does not make them zero. Where a tile has keys that some rows see and some do
 // not, the products take its values without those, and each row adds the ones that it sees: its sum is not finite either way.
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));

@@ -271,7 +271,9 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
   f32x16 acc[BLOCKS];
 #pragma unroll
   for (int i = 0; i < BLOCKS; ++i) acc[i] = f32x16{};
-  // a score's exponent is s scale - base; exponents above `margin` move the base: the first one, then those above 8
+  // a score's exponent is s scale - base; exponents above `margin` move the base, to LIFT below them: the first one, then
+  // those 8 above that
+  constexpr float BEGUN = LIFT<BF> + 8.0f;
   float base = 0.0f, margin = -INFINITY, total = 0.0f;
   u32x4 pf[4];
 
@@ -296,7 +298,7 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
     top = fmaxf(fmaxf(top, v[e]), v[e + 1]);
   };
   // Masks the exponents of tile u, whose largest is `top` before that, and settles the base: it moves only when a weight would
-  // exceed 2^8, and then exponents, acc and total with it.
+  // exceed its first by 2^8, and then exponents, acc and total with it.
   const auto settle = [&](f32x16(&s)[2], float top, int u) {
     const int key0 = (first + u) * PROMPT_TILE;
     if (key0 < all_low || key0 + PROMPT_TILE > all_limit) {
@@ -311,8 +313,8 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
     }
     if (__builtin_amdgcn_ballot_w64(top > margin) != 0) {
       top = pair_max(top);
-      const bool moves = top > margin, began = margin == 8.0f;
-      const float by = moves ? top : 0.0f, corr = moves && began ? __builtin_amdgcn_exp2f(-by) : 1.0f;
+      const bool moves = top > margin, began = margin == BEGUN;
+      const float by = moves ? top - LIFT<BF> : 0.0f, corr = moves && began ? __builtin_amdgcn_exp2f(-by) : 1.0f;
       total *= corr;
 #pragma unroll
       for (int i = 0; i < BLOCKS; ++i)
@@ -321,7 +323,7 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[0][r] -= by, s[1][r] -= by;
       base += by;
-      margin = moves ? 8.0f : margin;
+      margin = moves ? BEGUN : margin;
     }
   };
   // Tile u has keys that some rows see and some do not: if values of it are not finite, which every wave looks for in what it
@@ -465,7 +467,7 @@ __device__ __forceinline__ void prompt_tile(const PromptCall& c, const PromptTil
         *reinterpret_cast<f32x4*>(at + i * 32 + gq * 8) =
             f32x4{acc[i][gq * 4], acc[i][gq * 4 + 1], acc[i][gq * 4 + 2], acc[i][gq * 4 + 3]};
     if (half == 0) {
-      plane[PROMPT_ROWS * D + (wave * 32 + r32) * 2] = margin == 8.0f ? base : -INFINITY;
+      plane[PROMPT_ROWS * D + (wave * 32 + r32) * 2] = margin == BEGUN ? base : -INFINITY;
       plane[PROMPT_ROWS * D + (wave * 32 + r32) * 2 + 1] = total;
     }
     return;

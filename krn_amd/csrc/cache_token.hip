@@ -11,8 +11,8 @@
 // A wave computes S^T = K Q^T and O^T += V^T P^T with 16x16x32 MFMAs on its own tiles. A lane then holds one query row
 // (lane & 15) and eight keys of a tile: keys 4 g + r and 16 + 4 g + r, g = lane / 16, which are also the eight that it gives
 // the second product, so P goes from registers to registers. The maximum is exchanged between lanes only when a row exceeds the
-// running one by more than 2^8 in weight. P is kept in two 16-bit parts (2^-17 of a weight or less is left): the matrix cores
-// are idle nine tenths of the time.
+// running one by more than 2^8 in weight. P is kept in two 16-bit parts (what is left: 2^-17 of a weight in bf16; 2^-23 in f16,
+// or 2^-32 of the largest weight if that is more): the matrix cores are idle nine tenths of the time.
 //
 // K and V tiles come into LDS by direct loads, one buffer each a wave and no barrier: K's next tile leaves when this one's
 // fragments are in registers, V's likewise, so 8 to 16 KiB a wave are always on their way. The loads are non-temporal: a step
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES, 2) void cache_tokens(TokenCall c)
   };
 
   f32x4 acc[NB][D / 16];
-  float m[NB], base[NB], total[NB];  // base: m, or 0 while no key has been seen
+  float m[NB], base[NB], total[NB];  // weights are 2^(x - base), base = m - LIFT; m = -inf while no key has been seen
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     m[b] = -INFINITY, base[b] = 0.0f, total[b] = 0.0f;
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES, 2) void cache_tokens(TokenCall c)
         total[b] *= corr;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) acc[b][i] *= corr;
-        m[b] = next, base[b] = to_base;
+        m[b] = next, base[b] = to_base - LIFT<BF>;
       }
       float sum = 0.0f;
 #pragma unroll

@@ -1,0 +1,72 @@
+"""The softmax weights of attention over a paged cache where their 16-bit forms could lose them: many small ones beside a
+large one. Keys and values repeat every sixteen keys, so wherever the keys are shared out, each share has the large weights too."""
+
+import numpy as np
+import pytest
+
+from krn_amd.lib import cache_attention
+from oracle import cache as oracle
+from tests.paged import HALF_STEP, TINY, Paged, assert_within, values, words
+
+# packed, lengths, counts of new tokens, heads, kv_heads, d
+FORMS = [
+    (True, [16], [1], 1, 1, 64), (True, [3040], [40], 4, 2, 128), (True, [600, 39], [200, 31], 8, 2, 64), (True, [1000], [1000], 2, 1, 128),
+    (False, [16], [1], 1, 1, 64), (False, [1000], [1], 8, 2, 128), (False, [500, 33, 2], [3, 3, 3], 4, 4, 64),
+    (False, [1000, 64], [4, 4], 8, 1, 64), (False, [320] * 5, [1] * 5, 17, 1, 128),
+]  # fmt: skip
+# What a weight may be off by, relative, and near zero in units of the largest: f16 ones multiplied by
+# 2^7, so that half of their last step, 2^-25, is 2^-32 of the largest.
+ONE_PART = HALF_STEP
+NEAR_ZERO = {"bf16": 2.0**-133, "f16": 2.0**-32}
+
+
+def repeated(device, kind, lengths, kv_heads, d, keys, vals):
+    """A cache whose sequences have the rows `keys`, of the first columns, and one of `vals` in every column, again and again."""
+    def fill_keys(rng, shape):
+        k = np.zeros(shape)
+        k[:, :, : keys.shape[1]] = keys[: shape[1]]
+        return k
+
+    def fill_values(rng, shape):
+        return np.broadcast_to(vals[: shape[1], None], shape)
+
+    return Paged(device, np.random.default_rng(1), kind, lengths, kv_heads=kv_heads, d=d, fill=(fill_keys, fill_values))
+
+
+def sinks(device, kind, lengths, kv_heads, d):
+    """One key in sixteen has the weight 1 and the value 0, the others the weight e^-17.625, below 2^-25, and the value 1000."""
+    keys = np.zeros((16, 1))
+    keys[0] = 17.625
+    return repeated(device, kind, lengths, kv_heads, d, keys, np.where(np.arange(16) == 0, 0.0, 1000.0))
+
+
+def queries(kind, tokens, heads, d, columns):
+    q = np.zeros((tokens, heads, d))
+    q[:, :, :columns] = 1
+    return words(q, kind)
+
+
+def starts_of(counts):
+    return [0, *np.cumsum(counts).tolist()]
+
+
+def rounded(y, bound, kind):
+    return y, bound + (np.abs(y) + bound) * HALF_STEP[kind] + TINY[kind]
+
+
+def call(paged, packed, counts, q, **kwargs):
+    sequences = paged.sequences(starts=starts_of(counts)) if packed else paged.sequences(new=counts[0])
+    return values(cache_attention(paged.tensor(q), paged.cache, sequences, **kwargs))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("packed,lengths,counts,heads,kv_heads,d", FORMS)
+def test_many_small_weights_count_beside_a_large_one(device, kind, packed, lengths, counts, heads, kv_heads, d):
+    """A token sees at most fifteen small weights for each large one: what they lose near zero is 15 * 1000 of it."""
+    paged = sinks(device, kind, lengths, kv_heads, d)
+    q, exact = queries(kind, sum(counts), heads, d, 1)
+    got = call(paged, packed, counts, q, scale=1.0)
+    y, bound = oracle.attention(exact, np.nan_to_num(paged.keys), np.nan_to_num(paged.values), starts_of(counts), lengths,
+                                paged.table, 1.0, weight=ONE_PART[kind])
+    assert_within(got, *rounded(y, bound + 15 * 1000 * NEAR_ZERO[kind], kind))
