@@ -1,5 +1,8 @@
 """The softmax weights of attention over a paged cache where their 16-bit forms could lose them: many small ones beside a
-large one. Keys and values repeat every sixteen keys, so wherever the keys are shared out, each share has the large weights too."""
+large one, and sums that nearly cancel, which show whether a weight has one 16-bit part or two. Keys and values repeat every
+sixteen keys, so wherever the keys are shared out, each share has the large weights too."""
+
+import math
 
 import numpy as np
 import pytest
@@ -14,9 +17,10 @@ FORMS = [
     (False, [16], [1], 1, 1, 64), (False, [1000], [1], 8, 2, 128), (False, [500, 33, 2], [3, 3, 3], 4, 4, 64),
     (False, [1000, 64], [4, 4], 8, 1, 64), (False, [320] * 5, [1] * 5, 17, 1, 128),
 ]  # fmt: skip
-# What a weight may be off by, relative, and near zero in units of the largest: f16 ones multiplied by
+# What a weight may be off by, relative, and near zero in units of the largest: one 16-bit part or two, f16 ones multiplied by
 # 2^7, so that half of their last step, 2^-25, is 2^-32 of the largest.
 ONE_PART = HALF_STEP
+TWO_PARTS = {"bf16": 2.0**-17, "f16": 2.0**-23}
 NEAR_ZERO = {"bf16": 2.0**-133, "f16": 2.0**-32}
 
 
@@ -38,6 +42,23 @@ def sinks(device, kind, lengths, kv_heads, d):
     keys = np.zeros((16, 1))
     keys[0] = 17.625
     return repeated(device, kind, lengths, kv_heads, d, keys, np.where(np.arange(16) == 0, 0.0, 1000.0))
+
+
+def halves(kind):
+    """A weight just below the middle between one half and the type's next value, and the logarithm as a sum of its values."""
+    weight, parts = 0.5 * (1 + 0.98 * HALF_STEP[kind]), []
+    left = math.log(weight)
+    for _ in range(4):
+        parts.append(float(words(np.array([left]), kind)[1][0]))
+        left -= parts[-1]
+    return weight, parts
+
+
+def cancelling(device, kind, lengths, kv_heads, d):
+    """Keys in turns of the weight 1 and the value 1, and of a weight that one part rounds to 1/2 and the value -2."""
+    keys = np.zeros((16, 4))
+    keys[1::2] = halves(kind)[1]
+    return repeated(device, kind, lengths, kv_heads, d, keys, np.where(np.arange(16) % 2 == 0, 1.0, -2.0))
 
 
 def queries(kind, tokens, heads, d, columns):
@@ -70,3 +91,38 @@ def test_many_small_weights_count_beside_a_large_one(device, kind, packed, lengt
     y, bound = oracle.attention(exact, np.nan_to_num(paged.keys), np.nan_to_num(paged.values), starts_of(counts), lengths,
                                 paged.table, 1.0, weight=ONE_PART[kind])
     assert_within(got, *rounded(y, bound + 15 * 1000 * NEAR_ZERO[kind], kind))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("packed,lengths,counts,heads,kv_heads,d", [form for form in FORMS if not form[0]])
+def test_weights_of_new_tokens_have_two_parts(device, kind, packed, lengths, counts, heads, kv_heads, d):
+    paged = cancelling(device, kind, lengths, kv_heads, d)
+    q, exact = queries(kind, sum(counts), heads, d, 4)
+    assert_within(call(paged, packed, counts, q, scale=1.0), *rounded(*oracle.attention(
+        exact, np.nan_to_num(paged.keys), np.nan_to_num(paged.values), starts_of(counts), lengths, paged.table, 1.0,
+        weight=TWO_PARTS[kind], tiny=NEAR_ZERO[kind]), kind))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("n", [16, 320, 1000])
+def test_one_part_is_more_than_two_parts_may_be_off(kind, n):
+    """On the host: weights of one part give zero where the test above accepts no such thing. (The logarithm's last part is off
+    by half of f16's last step, 2^-25.)"""
+    paged = cancelling(None, kind, [n], 1, 64)
+    _, exact = queries(kind, 1, 1, 64, 4)
+    y, bound = rounded(*oracle.attention(exact, paged.keys, paged.values, [0, 1], [n], paged.table, 1.0, weight=TWO_PARTS[kind],
+                                         tiny=NEAR_ZERO[kind]), kind)
+    weight = halves(kind)[0]
+    np.testing.assert_allclose(y, (1 - 2 * weight) / (1 + weight), rtol=0, atol=2.0**-25)
+    one = words(np.array([weight]), kind)[1][0]
+    assert one == 0.5 and (np.abs((1 - 2 * one) / (1 + weight) - y) > bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("packed,lengths,counts,heads,kv_heads,d", FORMS)
+def test_scores_of_minus_infinity_alone_give_zeros(device, kind, packed, lengths, counts, heads, kv_heads, d):
+    paged = repeated(device, kind, lengths, kv_heads, d, np.full((16, 1), -np.inf), np.ones(16))
+    got = call(paged, packed, counts, queries(kind, sum(counts), heads, d, 1)[0])
+    np.testing.assert_array_equal(got, np.zeros(got.shape))
