@@ -228,7 +228,9 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES, 2) void cache_tokens(TokenCall c)
   const int seq = share.seq, part = share.part, parts = share.parts;
   const int t = threadIdx.x, lane = t & 63, g = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  if (parts > 1 && part == 0 && kv == 0 && t == 0) c.header[1 + share.order] = {seq, w, parts, 0};
+  // parts of the sequences in several before this one: all parts, less the sequences in one
+  const int place = w - (seq - share.order);
+  if (parts > 1 && part == 0 && kv == 0 && t == 0) c.header[1 + share.order] = {seq, place, parts, 0};
 
   const int length = __builtin_amdgcn_readfirstlane(sequence_length(c.s, seq)), end = held_keys(c.s, length, c.cache.page_shift);
   const TileRange range = tiles_of(c, length);
@@ -413,7 +415,7 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES, 2) void cache_tokens(TokenCall c)
 
   // the waves' rows meet in LDS, sixteen at a time: a lane has columns i * 16 + 4 g to + 3 of its row
   float* mine = reinterpret_cast<float*>(kbuf);
-  float* plane = c.planes + ((int64_t)w * c.cache.kv_heads + kv) * c.rows * (D + 4);
+  float* plane = c.planes + ((int64_t)place * c.cache.kv_heads + kv) * c.rows * (D + 4);
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     if (b * 16 >= c.rows) break;
@@ -516,7 +518,8 @@ TokenPlan krn::token_plan(int64_t step, int64_t group, int64_t kv_heads, int64_t
   p.joins = sequences < extra ? sequences : extra;
   p.header_bytes = p.split ? (p.joins + 1) * 16 : 0;
   p.map_bytes = p.mapped ? p.workgroups * 16 : 0;
-  p.bytes = p.split ? p.header_bytes + p.map_bytes + p.workgroups * kv_heads * p.rows * (d + 4) * 4 : 0;
+  // planes of the parts beyond the first, and of the first ones of the sequences that have those
+  p.bytes = p.split ? p.header_bytes + p.map_bytes + (extra + p.joins) * kv_heads * p.rows * (d + 4) * 4 : 0;
   return p;
 }
 
