@@ -12,6 +12,7 @@ from krn_amd.runtime import library
 from krn_amd.runtime.hip import HIPDevice, HIPTensor
 
 HEADS = (64, 128)  # head dimensions
+ALL_KEYS = 2**31  # a window that holds any sequence
 
 
 class KvCache:
@@ -186,7 +187,7 @@ def cache_attention(q, cache: KvCache, sequences: Sequences, *, scale: float | N
     sizes = (tokens, heads, *cache.sizes)
     need = library.cache_attention_workspace(*sizes, *sequences.arguments)
     call = library.cache_attention_call(cache.dtype, q.pointer, *cache.pointers, result.pointer, *sizes, *sequences.arguments,
-                                        scale if scale is not None else d**-0.5, window or 0, need)
+                                        scale if scale is not None else d**-0.5, min(window or 0, ALL_KEYS), need)
 
     def run(stream) -> None:
         if need:
