@@ -206,7 +206,8 @@ int krn_rotary_append(int kind, const void* qkv, void* q, void* keys, void* valu
  * if that is not 0. q and o are tokens x heads x d; heads / kv_heads query heads share a key head; scale > 0. A token without
  * keys gets zeros. Keys and values that a token does not see have no part in its result, NaN and infinities included; pages that
  * lie wholly before the windows of all new tokens may belong to other sequences. Weights are rounded to 16 bits before they
- * multiply values, to two 16-bit parts without starts and with up to 32 rows (step * heads / kv_heads). o may be q itself and
+ * multiply values, to two 16-bit parts without starts and with up to 32 rows (step * heads / kv_heads); in KRN_F16, weights
+ * below 2^-32 of a token's largest are lost. A token whose scores are all minus infinity gets zeros. o may be q itself and
  * shares no other memory. A workspace of krn_cache_attention_workspace bytes (`packed`: with starts; 16-byte aligned, no
  * preparation, not touched by other work until this call's has run; calls on one stream may share one) lets the keys of one
  * token be split over workgroups; with less, or none, they stay in one. */

@@ -94,8 +94,11 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 
 // Attention of new tokens, a few of every sequence (cache_token.hip)
 constexpr int TOKEN_WAVES = 4;
-// Rows of a key head, at most; more are a prompt's. (64 sequences of 4000 keys, d = 128, 8 key heads: 32 rows 207 us here
-// and 189 there, but one sequence 12 and 24; 64 rows, in two more blocks of sixteen, 270 and 193, one sequence 20 and 24.)
+// Rows of a key head, at most; more are a prompt's. What is faster hangs on the batch, which this rule does not look at: it is
+// set for large ones and costs small ones of 33 to 64 rows up to half of their time. (d = 128, 8 key heads, here and there:
+// 64 sequences of 4000 keys, 32 rows 207 and 189 us, 64 rows, in two more blocks of sixteen, 270 and 193; one sequence of
+// 4000, 32 rows 12 and 24, 48 rows 20 and 37, 64 rows 20 and 24, of 500 and 48 rows 16 and 25. One key head, 8 sequences of
+// 2000, 40 and 64 rows: 16 and 25, 18 and 26.)
 constexpr int TOKEN_ROWS = 32;
 // Parts that the keys of all sequences and columns are shared out to: two for each workgroup that runs at once. (64 sequences of
 // 4096 keys on average, d = 128: 512 parts 179 us, 1024 173, 2048 176; of 4096 each 164, 170, 175; 2 of 131000 103, 99, 102.)
@@ -144,7 +147,7 @@ constexpr int PROMPT_CHUNK = 16;
 // with a prompt of 2000 tokens, would run on alone (891 us, shared out 131). Counting parts and the joining launch cost 60
 // prompts of 150 tokens with such a table 53.0 and 56.7.
 constexpr int PROMPT_LONG = 128;
-constexpr int PROMPT_CUS = 512;  // workgroups that run at once
+constexpr int PROMPT_PLACES = 512;  // workgroups that run at once, two a CU
 
 struct PromptCall {
   const uint16_t* q;

@@ -87,9 +87,12 @@ __device__ __forceinline__ KeyTiles tiles_seen(const PromptCall& c, const TokenR
 
 // Rows before many keys are shared out: workgroup w of a column does part `part` of `parts` of a tile of rows. All tiles of
 // rows of a sequence have as many parts, so that nothing loops over them: with R of them of up to T key tiles each, ceil(T
-// / chunk), and chunk is the sum of all R T over `spare`, the workgroups that are there beyond one for each tile of rows.
-// Every wave counts for itself, a lane for ceil(n / 64) sequences in a row. What no chip does in a second stays whole, and
-// the sums below 2^32.
+// / chunk), and chunk is the sum of all R T over `spare`, the workgroups that are there beyond one for each tile of rows. That
+// sum has the rows that stay whole in it too, so a few long rows beside many short ones are in fewer parts than there are
+// workgroups for (1 token after 65000 keys 62 us, 2000 tokens 47, packed together 123).
+// Every wave counts for itself, a lane for ceil(n / 64) sequences in a row. Sequences of R T above 2^22 (16 ms of the whole
+// chip a key head at d = 128, half of that for a prompt) stay whole and are not counted, which keeps the sum over up to
+// 512 sequences in 32 bits.
 struct PromptPart {
   int part, parts, plane, order;  // plane: of the first part, among all planes; order: of the rows, among those in several parts
 };
@@ -562,7 +565,7 @@ PromptPlan krn::prompt_plan(int64_t tokens, int64_t step, int64_t group, int64_t
   p.slots = p.workgroups = step > 0 ? sequences * ((step * group + PROMPT_ROWS - 1) / PROMPT_ROWS)
                                     : tokens * group / PROMPT_ROWS + sequences;
   // parts beyond the first of all tiles of rows, in each column: as many as run at once without them, or half of that
-  const int64_t at_once = PROMPT_CUS / kv_heads, tiles = width * page / PROMPT_TILE;
+  const int64_t at_once = PROMPT_PLACES / kv_heads, tiles = width * page / PROMPT_TILE;
   if (at_once == 0 || tiles <= PROMPT_CHUNK || (p.slots >= at_once && (tiles <= PROMPT_LONG || sequences > 256))) return p;
   const int64_t header = (at_once + 1) * 16, need = header + 2 * at_once * kv_heads * PROMPT_ROWS * (d + 2) * 4;
   if (need > bytes) return p;

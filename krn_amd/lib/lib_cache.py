@@ -107,7 +107,8 @@ class Rotary:
            interleaved: bool = False) -> "Rotary":
         """frequencies[j] = base^(-2j / dim), for contexts `factor` times as long as those of training: all of them divided
         by `factor` or, with the `original` context length, only those of pairs that turn less than once in it, those beyond
-        32 turns as they are and a linear mix between (with the magnitude 0.1 ln factor + 1 that goes with it)."""
+        32 turns as they are and between these a mix linear in the turns, with the magnitude 0.1 ln factor + 1. Models whose
+        mix is linear in the pair's index, or that have other limits or magnitudes, pass theirs to `Rotary` itself."""
         if not isinstance(dim, int) or dim < 0 or dim % 2:
             raise ValueError(f"an even number of columns is rotated, not {dim!r}")
         if not (math.isfinite(base) and base > 0 and math.isfinite(factor) and factor >= 1):
@@ -169,8 +170,10 @@ def cache_attention(q, cache: KvCache, sequences: Sequences, *, scale: float | N
     heads share a key head; scale is 1 / sqrt(d) unless given. A token without keys gets zeros. Keys and values that a token
     does not see have no part in its result, NaN and infinities included; pages wholly before the windows of all new tokens
     may be another sequence's. Scores, maxima and sums are float32; softmax weights are rounded to 16 bits before they multiply
-    values, to two 16-bit parts where sequences have up to 32 rows, new tokens times query heads of a key head. `out` may be q
-    itself and shares no other memory. Sequences of as many new tokens each, a few, are faster without `starts`."""
+    values, to two 16-bit parts where sequences have up to 32 rows, new tokens times query heads of a key head; in f16, weights
+    below 2^-32 of a token's largest are lost. A token whose scores are all minus infinity gets zeros too. `out` may be q itself and
+    shares no other memory. Sequences of as many new tokens each, a few, are faster without `starts`, and new tokens with a long
+    past are faster in a call of their own than packed beside prompts."""
     _checked(cache, sequences)
     tensor(q, "q", 3, (cache.dtype,))
     tokens, heads, d = q.shape
