@@ -126,7 +126,7 @@ struct TokenCall {
   uint32_t shares;  // the parts of a key head, with all sequences in one row
   int4* header;     // the number of sequences in several parts, then of each (sequence, first plane, parts, -)
   int4* map;        // of a workgroup (sequence or -1, part, parts, order of a sequence in several), if counted before
-  float* planes;    // of a part of a sequence in several, and key head: `rows` rows of sums, then their maxima and sums of weights
+  float* planes;    // of a part of a sequence in several, and key head: `rows` rows of sums, then their bases and sums of weights
 };
 
 // rows: of a key head

@@ -310,10 +310,12 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES, 2) void cache_tokens(TokenCall c)
   };
 
   f32x4 acc[NB][D / 16];
-  float m[NB], base[NB], total[NB];  // weights are 2^(x - base), base = m - LIFT; m = -inf while no key has been seen
+  // weights are 2^(x - base); exponents above `margin` move the base, to LIFT below them: the first one, then those 8 above that
+  constexpr float BEGUN = LIFT<BF> + 8.0f;
+  float base[NB], margin[NB], total[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    m[b] = -INFINITY, base[b] = 0.0f, total[b] = 0.0f;
+    base[b] = 0.0f, margin[b] = -INFINITY, total[b] = 0.0f;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) acc[b][i] = f32x4{};
   }
@@ -354,14 +356,16 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES, 2) void cache_tokens(TokenCall c)
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);
-      // the base moves only when a weight would exceed 2^8: then maxima meet, and acc and total are rescaled
-      if (__builtin_amdgcn_ballot_w64(top > m[b] + 8.0f) != 0) {
-        const float next = fmaxf(m[b], row_max(top)), to_base = next == -INFINITY ? 0.0f : next;
-        const float corr = __builtin_amdgcn_exp2f(m[b] - to_base);
+      // the base moves only when a weight would exceed its first by 2^8: then maxima meet, and acc and total are rescaled. What
+      // is compared is the rounded exponent, so that no weight exceeds 2^15, f16's range, however large the scores are
+      if (__builtin_amdgcn_ballot_w64(top - base[b] > margin[b]) != 0) {
+        const float most = row_max(top);
+        const bool moves = most - base[b] > margin[b], began = margin[b] == BEGUN;
+        const float next = moves ? most - LIFT<BF> : base[b], corr = began ? __builtin_amdgcn_exp2f(base[b] - next) : 1.0f;
         total[b] *= corr;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) acc[b][i] *= corr;
-        m[b] = next, base[b] = to_base - LIFT<BF>;
+        base[b] = next, margin[b] = moves ? BEGUN : margin[b];
       }
       float sum = 0.0f;
 #pragma unroll
@@ -421,7 +425,7 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES, 2) void cache_tokens(TokenCall c)
     if (b * 16 >= c.rows) break;
     const float sum = row_sum(total[b]);
     __syncthreads();  // every wave is done with its tiles, or with the rows before
-    if (g == 0) stat[0][wave][col] = m[b], stat[1][wave][col] = sum;
+    if (g == 0) stat[0][wave][col] = margin[b] == BEGUN ? base[b] : -INFINITY, stat[1][wave][col] = sum;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(mine + col * OLD + i * 16 + g * 4) = acc[b][i];
     __syncthreads();
@@ -439,7 +443,7 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES, 2) void cache_tokens(TokenCall c)
         all += f * stat[1][x][row];
         o += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * 2 * TILE) + row * OLD + d);
       }
-      if (parts > 1) {  // unnormalised rows, then their maxima and sums
+      if (parts > 1) {  // unnormalised rows, then their bases and sums
         const int r = b * 16 + row;
         *reinterpret_cast<f32x4*>(plane + r * D + d) = o;
         if (d == 0) plane[c.rows * D + r * 2] = top, plane[c.rows * D + r * 2 + 1] = all;

@@ -126,3 +126,28 @@ def test_scores_of_minus_infinity_alone_give_zeros(device, kind, packed, lengths
     paged = repeated(device, kind, lengths, kv_heads, d, np.full((16, 1), -np.inf), np.ones(16))
     got = call(paged, packed, counts, queries(kind, sum(counts), heads, d, 1)[0])
     np.testing.assert_array_equal(got, np.zeros(got.shape))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("size", [1e5, 3e7, 7e7, 1e8, 2e8])
+@pytest.mark.parametrize("packed,lengths,counts,heads,kv_heads,d", FORMS)
+def test_scores_whose_steps_are_large_give_a_mean(device, kind, size, packed, lengths, counts, heads, kv_heads, d):
+    """Scores of up to 10^8 differ by float32's steps, 8 and 16 there: the weights are what they come to, but a mean of equal
+    values is that value, off by a weight's rounding, of n sums' 2^-23 (n + 64), and the result's."""
+    rng = np.random.default_rng(int(size) % 1009)
+    vals = rng.integers(1, 9, d).astype(float)
+
+    def fill_keys(rng, shape):
+        k = np.zeros(shape)
+        k[:, :, 0], k[:, :, 1] = size / 30000, rng.integers(0, 60, shape[:2])
+        return k
+
+    paged = Paged(device, rng, kind, lengths, kv_heads=kv_heads, d=d, fill=(fill_keys, lambda rng, shape: np.broadcast_to(vals, shape)))
+    q = np.zeros((sum(counts), heads, d))
+    q[:, :, 0], q[:, :, 1] = rng.integers(25000, 32000, q.shape[:2]), rng.integers(-1, 2, q.shape[:2])
+    got = call(paged, packed, counts, words(q, kind)[0], scale=1.0)
+    n = max(lengths)
+    _, position = oracle.owners(starts_of(counts), lengths, sum(counts))
+    want = np.broadcast_to(vals, got.shape) * (position >= 0)[:, None, None]  # a token before all keys has none
+    assert_within(got, *rounded(want, want * (ONE_PART[kind] + n * NEAR_ZERO[kind] + (n + 64) * 2.0**-23), kind))
